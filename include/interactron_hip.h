@@ -531,6 +531,41 @@ int ix_sumsq_accum_f32(const float* x, int64_t n, float* out, void* workspace, s
 int ix_adam_step_f32(float* p, float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
                      int step, const float* sumsq, float max_norm, int zero_grad, ix_stream_t stream);
 
+/* ---- A paged cache of keys and values (csrc/cache.hip): acting on a rollout that grows token by token --------------------------------
+ * The reference runs its fusion transformer over the whole sequence again for every new frame (models/transformer.py:49-60,
+ * models/interactron.py:166-190); these entry points keep what has been seen.  Token t of sequence b and key head h lives at row
+ * t % page of page table[b][t / page] in pools k, v [pages_total][kv_heads][page][hd].  dtype: 0 f32, 1 bf16, 2 fp16; hd 32, 64 or
+ * 128; page a power of two, 16 .. 1024.  lens [batch]: tokens held (clamped to 0 .. pages * page).  weight [batch][kv_heads]
+ * [pages * page] f32 (may be null): attention that every token has had so far.  A page id outside the pool is never dereferenced: its
+ * tokens count as masked, what is written there is dropped.  Strides are in elements, rows start on 16 bytes.
+ *   ix_cache_append : rows k, v [batch][T][kv_heads][hd] -> tokens at[b] .. at[b] + counts[b] - 1 (null: the lengths; T), their weight
+ *                     = 0, lens[b] = at[b] + counts[b]; tokens beyond the capacity are dropped
+ *   ix_cache_attn   : out[b][h] = sum_j P_j v_j, P = softmax_j(scale q[b][h] . k_j) for one query per sequence and head that stands at
+ *                     the last token; window > 0: the last `window` tokens and the first `sinks` only.  Query head h reads key head
+ *                     h / (heads / kv_heads).  accumulate: weight[j] += sum of P_j over the query heads of the key head.  An empty
+ *                     sequence gives zeros.  f32 sums; split over the length, joined in split order (no atomics)
+ *   ix_cache_select : kept [batch][kv_heads][budget], ascending: the first `sinks`, the last `recent` tokens and of the rest those of
+ *                     the largest weight (NaN counts least; of equal weights the lowest index); all tokens, then -1, where there are
+ *                     no more than `budget`.  left[b] = min(lens[b], budget)
+ *   ix_cache_compact: rows kept[b][h][i] >= i (ascending; others are skipped) -> rows i < left[b], in place, with their weights;
+ *                     lens = left */
+struct ix_paged_cache {
+    void *k, *v;
+    const int* table;
+    int* lens;
+    float* weight;
+    int64_t pages_total;
+    int dtype, kv_heads, page, hd, batch, pages;
+};
+int ix_cache_append(const struct ix_paged_cache* cache_host, const void* k, const void* v, int T, int64_t sb_k, int64_t st_k, int64_t sh_k,
+                    int64_t sb_v, int64_t st_v, int64_t sh_v, const int* counts, const int* at, ix_stream_t stream);
+int ix_workspace_bytes_cache_attn(const struct ix_paged_cache* cache_host, int heads, int window, int sinks, int accumulate, size_t* out_host);
+int ix_cache_attn(const struct ix_paged_cache* cache_host, const void* q, int64_t sq_b, int64_t sq_h, void* out, int heads, float scale,
+                  int window, int sinks, int accumulate, void* workspace, size_t workspace_bytes, ix_stream_t stream);
+int ix_cache_select(const float* weight, const int* lens, int* kept, int* left, int batch, int kv_heads, int capacity, int budget,
+                    int sinks, int recent, ix_stream_t stream);
+int ix_cache_compact(const struct ix_paged_cache* cache_host, const int* kept, const int* left, int budget, ix_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,210 @@
+"""hipops.cache -- a paged cache of keys and values for acting on a rollout that grows token by token: writing new tokens, attention of
+one new token per sequence, and cutting the cache back to the tokens that have had the most attention (csrc/cache.hip).
+
+    cache = hipops.PagedCache(k, v, table, lens, weight)      # tensors of the caller; nothing is copied
+    hipops.cache_append(cache, new_k, new_v)                  # [B, T, kv_heads, hd] each, at the end of every sequence
+    out = hipops.cache_attention(q, cache, accumulate=True)   # q [B, heads, hd] -> [B, heads, hd]
+    hipops.cache_evict(cache, budget, sinks=4, recent=256)    # in place; the pages behind the budget are free again
+
+None of these has a backward.  All of them are ordered on the current stream, never wait for the GPU, take their sizes from the shapes
+alone (the lengths stay on the device) and may be captured into a HIP graph.  (The reference keeps nothing: it runs its fusion transformer
+over all frames again for every new one, models/interactron.py:166-190.)
+"""
+import ctypes
+
+import torch
+
+from .. import _lib
+from . import core
+from .core import _L, _chk, _stream
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_HEAD_DIMS = (32, 64, 128)
+
+
+class _CacheC(ctypes.Structure):   # struct ix_paged_cache of include/interactron_hip.h
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("table", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+                ("weight", ctypes.c_void_p), ("pages_total", ctypes.c_int64), ("dtype", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("page", ctypes.c_int), ("hd", ctypes.c_int), ("batch", ctypes.c_int), ("pages", ctypes.c_int)]
+
+
+def _here(*named):
+    """The current stream, after checking that every (tensor, name) lives on the device this process computes on."""
+    for t, name in named:
+        if t is not None and not t.is_cuda:
+            raise _lib.HipLibraryError("%s must live on the GPU: the HIP path has no CPU fallback" % name)
+    s = _stream()
+    dev = core._dev[0] if core._dev[0] is not None else torch.cuda.current_device()
+    for t, name in named:
+        if t is not None and t.device.index != dev:
+            raise _lib.HipLibraryError("%s lives on cuda:%d but this process computes on cuda:%d (one process per GPU)" % (name, t.device.index, dev))
+    if torch.cuda.current_device() != dev:
+        raise _lib.HipLibraryError("the current device is cuda:%d but this process computes on cuda:%d (one process per GPU)" % (torch.cuda.current_device(), dev))
+    return s
+
+
+def _whole(t, name, dtype, shape):
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise ValueError("%s must be %s %s, got %s %s" % (name, dtype, list(shape), t.dtype, list(t.shape)))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous: it is used in place" % name)
+
+
+def _count(x, name, least=0):
+    if isinstance(x, bool) or not isinstance(x, int) or x < least or x >= 1 << 30:
+        raise ValueError("%s must be a whole number from %d to 2^30 - 1, got %r" % (name, least, x))
+    return x
+
+
+class PagedCache:
+    """Keys and values of `batch` sequences in pages of a shared pool.
+
+    k, v     [pages_total, kv_heads, page, hd], float32, bfloat16 or float16; hd 32, 64 or 128; page a power of two, 16 .. 1024
+    table    int32 [batch, pages]: the pages of every sequence in order; token t is row t % page of page table[b, t // page].  Entries
+             behind a sequence's length are not read; one that is outside the pool counts as masked and is never written through.  Two
+             sequences may share pages that both only read.
+    lens     int32 [batch]: tokens held
+    weight   float32 [batch, kv_heads, pages * page] or None: the attention each token has had so far
+    """
+    __slots__ = ("k", "v", "table", "lens", "weight", "kv_heads", "hd", "page", "batch", "pages", "capacity", "c", "ref", "_ws")
+
+    def __init__(self, k, v, table, lens, weight=None):
+        if k.dim() != 4 or k.dtype not in _DTYPES:
+            raise ValueError("cache keys must be [pages_total, kv_heads, page, hd] in float32, bfloat16 or float16, got %s %s" % (k.dtype, list(k.shape)))
+        total, kv, page, hd = k.shape
+        if hd not in _HEAD_DIMS:
+            raise ValueError("a cache of head dim %d: %s are supported" % (hd, _HEAD_DIMS))
+        if page < 16 or page > 1024 or page & (page - 1):
+            raise ValueError("a page of %d tokens: powers of two from 16 to 1024 are supported" % page)
+        if table.dim() != 2 or 0 in table.shape or 0 in k.shape:
+            raise ValueError("an empty cache, or a page table that is not [batch, pages]: %s, %s" % (list(k.shape), list(table.shape)))
+        B, pages = table.shape
+        _whole(k, "cache keys", k.dtype, (total, kv, page, hd))
+        _whole(v, "cache values", k.dtype, (total, kv, page, hd))
+        _whole(table, "the page table", torch.int32, (B, pages))
+        _whole(lens, "the lengths", torch.int32, (B,))
+        if weight is not None:
+            _whole(weight, "the weights", torch.float32, (B, kv, pages * page))
+        if B > 65535 or kv > 1024 or pages * page >= 1 << 30 or total >= 1 << 31:
+            raise ValueError("a cache of %d sequences, %d key heads, %d tokens a sequence is too large" % (B, kv, pages * page))
+        _here((k, "cache keys"), (v, "cache values"), (table, "the page table"), (lens, "the lengths"), (weight, "the weights"))
+        if k.data_ptr() % 16 or v.data_ptr() % 16:
+            raise ValueError("cache keys and values must start on 16 bytes")
+        self.k, self.v, self.table, self.lens, self.weight = k, v, table, lens, weight
+        self.kv_heads, self.hd, self.page, self.batch, self.pages, self.capacity = kv, hd, page, B, pages, pages * page
+        self.c = _CacheC(k.data_ptr(), v.data_ptr(), table.data_ptr(), lens.data_ptr(), weight.data_ptr() if weight is not None else None, total,
+                         _DTYPES[k.dtype], kv, page, hd, B, pages)
+        self.ref = ctypes.byref(self.c)
+        self._ws = {}   # workspace bytes by call signature
+
+
+def _rows(t, name, cache, shape, dims):
+    """t with rows that the kernels can read: last dimension dense, every row on 16 bytes (copied where it is not)"""
+    if t.dtype != cache.k.dtype or tuple(t.shape) != shape:
+        raise ValueError("%s must be %s %s like the cache, got %s %s" % (name, cache.k.dtype, list(shape), t.dtype, list(t.shape)))
+    per = 16 // t.element_size()
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(t.stride(d) % per for d in range(dims)):
+        t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _per_sequence(t, name, cache):
+    if t is not None:
+        _whole(t, name, torch.int32, (cache.batch,))
+    return t
+
+
+def cache_append(cache, k, v, counts=None, at=None):
+    """Writes k, v [B, T, kv_heads, hd] as tokens at[b] .. at[b] + counts[b] - 1 of every sequence and sets the lengths to at + counts.
+
+    at: int32 [B], default: the cache's lengths (the new tokens follow the old ones; an earlier place takes tokens back).  counts: int32
+    [B], default T (rows behind a sequence's count are padding and not read).  Tokens beyond the capacity are dropped.  New tokens have
+    had no attention yet: their weight is 0."""
+    if k.dim() != 4:
+        raise ValueError("new keys must be [batch, tokens, kv_heads, hd], got %s" % list(k.shape))
+    T = k.shape[1]
+    shape = (cache.batch, T, cache.kv_heads, cache.hd)
+    k, v = _rows(k, "new keys", cache, shape, 3), _rows(v, "new values", cache, shape, 3)
+    _per_sequence(counts, "counts", cache)
+    _per_sequence(at, "at", cache)
+    s = _here((k, "new keys"), (v, "new values"), (counts, "counts"), (at, "at"))
+    _chk(_L().ix_cache_append(cache.ref, k.data_ptr(), v.data_ptr(), T, *k.stride()[:3], *v.stride()[:3],
+                              counts.data_ptr() if counts is not None else None, at.data_ptr() if at is not None else None, s), "ix_cache_append")
+
+
+def cache_attention(q, cache, scale=None, window=None, sinks=0, accumulate=False):
+    """Attention of one new token per sequence: q [B, heads, hd] stands at the last token of its sequence -> [B, heads, hd].
+
+    heads is a multiple of the cache's kv_heads; head h reads key head h // (heads // kv_heads).  scale: default 1 / sqrt(hd).  window:
+    only the last `window` tokens and the first `sinks` are seen (default: all).  accumulate: the attention that every token gets here,
+    summed over the heads that share its key head, is added to cache.weight.  An empty sequence gives zeros."""
+    if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % cache.kv_heads:
+        raise ValueError("q must be [batch, heads, hd] with a multiple of %d heads, got %s" % (cache.kv_heads, list(q.shape)))
+    H = q.shape[1]
+    if H > 4096:
+        raise ValueError("%d query heads: at most 4096 are supported" % H)
+    q = _rows(q, "q", cache, (cache.batch, H, cache.hd), 2)
+    w, sinks = 0 if window is None else _count(window, "window", 1), _count(sinks, "sinks")
+    if accumulate and cache.weight is None:
+        raise ValueError("accumulate: the cache holds no weights")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise _lib.HipLibraryError("cache_attention has no backward: call it under torch.no_grad()")
+    s = _here((q, "q"))
+    key = (H, w, sinks, bool(accumulate))
+    need = cache._ws.get(key)
+    if need is None:
+        n = ctypes.c_size_t(0)
+        _chk(_L().ix_workspace_bytes_cache_attn(cache.ref, H, w, sinks, int(bool(accumulate)), ctypes.byref(n)), "ix_workspace_bytes_cache_attn")
+        need = cache._ws[key] = n.value
+    out = torch.empty((cache.batch, H, cache.hd), dtype=q.dtype, device=q.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None   # (a buffer per call: calls on other streams and captured graphs share none)
+    _chk(_L().ix_cache_attn(cache.ref, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), H, cache.hd ** -0.5 if scale is None else float(scale),
+                            w, sinks, int(bool(accumulate)), ws.data_ptr() if ws is not None else None, need, s), "ix_cache_attn")
+    return out
+
+
+def cache_select(weight, lens, budget, sinks=0, recent=0):
+    """The tokens that stay when sequences shrink to `budget`: weight [B, kv_heads, capacity], lens int32 [B] -> (kept, left).
+
+    kept int32 [B, kv_heads, budget], ascending: the first `sinks` tokens, the last `recent`, and of the rest those of the largest weight
+    (a NaN counts less than any number; of equal weights the lowest index stays).  left int32 [B] = min(lens, budget); a sequence that
+    is no longer than the budget keeps everything, and unused places of kept hold -1."""
+    if weight.dim() != 3 or weight.dtype != torch.float32 or 0 in weight.shape or not weight.is_contiguous():
+        raise ValueError("weight must be a contiguous float32 [batch, kv_heads, capacity], got %s %s" % (weight.dtype, list(weight.shape)))
+    B, kv, cap = weight.shape
+    if B > 65535 or cap >= 1 << 30:
+        raise ValueError("weights of %d sequences of %d tokens are too large" % (B, cap))
+    _whole(lens, "lens", torch.int32, (B,))
+    budget, sinks, recent = _count(budget, "budget", 1), _count(sinks, "sinks"), _count(recent, "recent")
+    if budget > cap or sinks + recent > budget:
+        raise ValueError("a budget of %d tokens for a capacity of %d, of which %d first and %d last ones" % (budget, cap, sinks, recent))
+    s = _here((weight, "weight"), (lens, "lens"))
+    kept = torch.empty((B, kv, budget), dtype=torch.int32, device=weight.device)
+    left = torch.empty(B, dtype=torch.int32, device=weight.device)
+    _chk(_L().ix_cache_select(weight.data_ptr(), lens.data_ptr(), kept.data_ptr(), left.data_ptr(), B, kv, cap, budget, sinks, recent, s), "ix_cache_select")
+    return kept, left
+
+
+def cache_compact(cache, kept, left):
+    """Moves the tokens kept[b, h, :left[b]] of every sequence and key head to its front, in place and in order, with their weights, and
+    sets the lengths to left.  kept int32 [B, kv_heads, budget] ascends in every row (as cache_select returns it); the pages of a
+    sequence must be its own: no other sequence's table may name them."""
+    if kept.dim() != 3 or kept.shape[2] == 0:
+        raise ValueError("kept must be [batch, kv_heads, budget], got %s" % list(kept.shape))
+    _whole(kept, "kept", torch.int32, (cache.batch, cache.kv_heads, kept.shape[2]))
+    _whole(left, "left", torch.int32, (cache.batch,))
+    if kept.shape[2] > cache.capacity:
+        raise ValueError("kept names %d tokens, the capacity is %d" % (kept.shape[2], cache.capacity))
+    if left.data_ptr() == cache.lens.data_ptr():
+        raise ValueError("left must not be the cache's own lengths")
+    s = _here((kept, "kept"), (left, "left"))
+    _chk(_L().ix_cache_compact(cache.ref, kept.data_ptr(), left.data_ptr(), kept.shape[2], s), "ix_cache_compact")
+
+
+def cache_evict(cache, budget, sinks=0, recent=0):
+    """Cuts every sequence back to `budget` tokens by the cache's own accumulated weights (cache_select + cache_compact) -> kept."""
+    if cache.weight is None:
+        raise ValueError("cache_evict: the cache holds no weights")
+    kept, left = cache_select(cache.weight, cache.lens, budget, sinks, recent)
+    cache_compact(cache, kept, left)
+    return kept
