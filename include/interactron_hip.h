@@ -531,6 +531,30 @@ int ix_sumsq_accum_f32(const float* x, int64_t n, float* out, void* workspace, s
 int ix_adam_step_f32(float* p, float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
                      int step, const float* sumsq, float max_norm, int zero_grad, ix_stream_t stream);
 
+/* ---- Band attention (csrc/band.hip): softmax(scale q k^T) v over a band around the diagonal and a few first keys ---------------------
+ * The sliding form of the attention of models/gpt.py:39-57 and models/detr_models/transformer.py:148-161 for rollouts whose [L, S] is
+ * too much: query i of a sequence of m queries and n keys stands at p = i + n - m and sees the keys j < n with |p - j| < window (0:
+ * all) or j < sinks; with `causal` also j <= p.  q [batch][Lq][heads][hd], k, v [batch][Lk][kv_heads][hd] by element strides (sb, sl,
+ * sh; rows dense and on 16 bytes); query head h reads key head h / (heads / kv_heads).  dtype 0 f32, 1 bf16, 2 fp16; hd 32, 64, 128.
+ * q_lens, kv_lens int32 [batch] (null: Lq, Lk): rows behind them are never read and come back as zeros.  A query that sees nothing
+ * gives zeros and has no gradient.  Keys and values that a query does not see have to be finite where they lie inside the lengths.
+ *   ix_band_attn_fwd : out [batch][Lq][heads][hd] dense; lse (may be null) f32 [batch][heads][pitch], base 2, for the gradients;
+ *                      pitch from ix_band_attn_lse_pitch
+ *   ix_band_attn_bwd : dq, dk, dv (dense, like q, k, v) from out, lse and d_out [batch][Lq][heads][hd] by strides g_*; sums in f32,
+ *                      in a fixed order (no atomics); workspace of ix_workspace_bytes_band_attn_bwd bytes, 16-byte aligned */
+struct ix_band {
+    const void *q, *k, *v;
+    int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
+    const int *q_lens, *kv_lens;
+    int dtype, batch, Lq, Lk, heads, kv_heads, hd, window, sinks, causal;
+    float scale;
+};
+int ix_band_attn_fwd(const struct ix_band* band_host, void* out, float* lse, ix_stream_t stream);
+int ix_band_attn_lse_pitch(int Lq, int64_t* out_host);
+int ix_workspace_bytes_band_attn_bwd(const struct ix_band* band_host, size_t* out_host);
+int ix_band_attn_bwd(const struct ix_band* band_host, const void* out, const float* lse, const void* d_out, int64_t g_sb, int64_t g_sl,
+                     int64_t g_sh, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, ix_stream_t stream);
+
 /* ---- A paged cache of keys and values (csrc/cache.hip): acting on a rollout that grows token by token --------------------------------
  * The reference runs its fusion transformer over the whole sequence again for every new frame (models/transformer.py:49-60,
  * models/interactron.py:166-190); these entry points keep what has been seen.  Token t of sequence b and key head h lives at row

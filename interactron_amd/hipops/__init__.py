@@ -14,6 +14,7 @@ The package is split by concern (round 6; it was one 2 800-line module):
     elementwise    elementwise / broadcast / reduction Functions, dropout, softmax, LayerNorm
     convolution    frozen-BN affines, fused contraction + BN, implicit-GEMM convolutions
     attn           materialised and flash attention, operand planes, key biases
+    band           attention over a band around the diagonal and a few first keys, with its gradients
     cache          paged cache of keys and values: append, attention of one new token, eviction
     criterion_ops  matcher cost, assignment, set criterion, policy cross-entropy, position embedding
     meta_ops       multi-tensor MAML plumbing and the fused outer step
@@ -28,9 +29,9 @@ COMPUTE_DTYPE) live in exactly one part each and are read and written THROUGH th
 import sys
 import types
 
-from . import core, elementwise, contraction, convolution, attn, cache, criterion_ops, meta_ops
+from . import core, elementwise, contraction, convolution, attn, band, cache, criterion_ops, meta_ops
 
-_PARTS = (core, elementwise, contraction, convolution, attn, cache, criterion_ops, meta_ops)
+_PARTS = (core, elementwise, contraction, convolution, attn, band, cache, criterion_ops, meta_ops)
 _SWITCH = {}    # name -> the part that owns a rebindable scalar
 _OWNER = {}     # name -> the part that defines a function / class / container
 for _m in _PARTS:

@@ -1,0 +1,115 @@
+"""hipops.band -- attention over a band around the diagonal and a few first keys, with its gradients (csrc/band.hip).
+
+The sliding form of hipops.attention for rollouts that are too long to attend to in full (reference models/gpt.py:39-57 and
+models/detr_models/transformer.py:148-161 attend to everything): 16-bit or 32-bit rows as they are, shared key heads, padded batches.
+"""
+import ctypes
+import math
+
+import torch
+
+from .. import _lib
+from .cache import _DTYPES, _HEAD_DIMS, _count, _here
+from .core import Function, _L, _NullCtx, _chk
+
+
+class _BandC(ctypes.Structure):   # struct ix_band of include/interactron_hip.h
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v")] +
+                [("%s_s%s" % (t, d), ctypes.c_int64) for t in "qkv" for d in "blh"] +
+                [("q_lens", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p)] +
+                [(n, ctypes.c_int) for n in ("dtype", "batch", "Lq", "Lk", "heads", "kv_heads", "hd", "window", "sinks", "causal")] +
+                [("scale", ctypes.c_float)])
+
+
+def _dense_rows(t):
+    """t, or a copy whose rows the kernels can read: last dimension dense, every row on 16 bytes"""
+    per = 16 // t.element_size()
+    sb, sl, sh, sd = t.stride()
+    if sd != 1 or sb % per or sl % per or sh % per or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _band(q, k, v, how):
+    window, sinks, causal, scale, q_lens, kv_lens = how
+    B, Lq, H, D = q.shape
+    c = _BandC(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+               q_lens.data_ptr() if q_lens is not None else None, kv_lens.data_ptr() if kv_lens is not None else None,
+               _DTYPES[q.dtype], B, Lq, k.shape[1], H, k.shape[2], D, window, sinks, causal, scale)
+    return ctypes.byref(c)
+
+
+class BandAttention(Function):
+    """(q, k, v) -> out; see band_attention.  Differentiable once (the sliding form is not part of the adaptation step, whose inner gradient
+    is differentiated again)."""
+    b16 = "native"
+
+    @staticmethod
+    def forward(ctx, q, k, v, q_lens, kv_lens, window, sinks, causal, scale):
+        how = (window, sinks, causal, scale, q_lens, kv_lens)
+        s = _here((q, "q"), (k, "k"), (v, "v"), (q_lens, "q_lens"), (kv_lens, "kv_lens"))
+        recorded = not isinstance(ctx, _NullCtx) and any(ctx.needs_input_grad[:3])
+        B, Lq, H, D = q.shape
+        ctx.how, ctx.shapes = how[:4], (q.shape, k.shape, v.shape)
+        ctx.empty = 0 in q.shape or k.shape[1] == 0
+        if ctx.empty:   # nothing to see: zeros, and no gradient
+            ctx.save_for_backward(q, k, v)
+            return q.new_zeros(q.shape)
+        q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
+        out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
+        lse = torch.empty((B, H, -(-Lq // 128) * 128), dtype=torch.float32, device=q.device) if recorded else None
+        _chk(_L().ix_band_attn_fwd(_band(q, k, v, how), out.data_ptr(), lse.data_ptr() if recorded else None, s), "ix_band_attn_fwd")
+        if recorded:
+            ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
+        return out
+
+    @staticmethod
+    def backward(ctx, do):
+        if torch.is_grad_enabled():   # (create_graph: a second derivative that silently left this node out would be a wrong one)
+            raise _lib.HipLibraryError("band_attention is differentiable once: no gradient of its gradient (create_graph=True)")
+        need = ctx.needs_input_grad
+        if ctx.empty:
+            return tuple(torch.zeros_like(t) if n else None for t, n in zip(ctx.saved_tensors, need)) + (None,) * 6
+        q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
+        do = _dense_rows(do.to(q.dtype))
+        s = _here((do, "the gradient"))
+        band = _band(q, k, v, ctx.how + (q_lens, kv_lens))
+        n = ctypes.c_size_t(0)
+        _chk(_L().ix_workspace_bytes_band_attn_bwd(band, ctypes.byref(n)), "ix_workspace_bytes_band_attn_bwd")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        _chk(_L().ix_band_attn_bwd(band, out.data_ptr(), lse.data_ptr(), do.data_ptr(), *do.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                   ws.data_ptr(), n.value, s), "ix_band_attn_bwd")
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None) + (None,) * 6
+
+
+def band_attention(q, k, v, window=None, sinks=0, causal=True, scale=None, q_lens=None, kv_lens=None):
+    """Attention of q [B, Lq, heads, hd] over k, v [B, Lk, kv_heads, hd] -> [B, Lq, heads, hd].
+
+    Query i of a sequence with m queries and n keys stands at p = i + n - m (the newest queries at the newest keys).  It sees the keys j
+    with |p - j| < window (default: all) and the first `sinks` ones; with `causal` only those up to p.  heads is a multiple of kv_heads;
+    head h reads key head h // (heads // kv_heads).  scale: default 1 / sqrt(hd).  q_lens, kv_lens: int32 [B], the lengths m and n of a
+    padded batch; padding is never read and comes back as zeros.  A query that sees nothing gives zeros and has no gradient.
+
+    float32, bfloat16 or float16 with sums and softmax in 32 bits, hd 32, 64 or 128, rows with any strides (a slice of a packed projection
+    is taken as it is).  Differentiable once.  Values have to be finite inside the lengths, also those a query does not see."""
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 4 or t.dtype not in _DTYPES or t.dtype != q.dtype:
+            raise ValueError("%s must be [batch, length, heads, hd] in float32, bfloat16 or float16 like q, got %s %s" % (name, t.dtype, list(t.shape)))
+    B, Lq, H, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError("k and v must be [%d, length, kv_heads, %d], got %s and %s" % (B, D, list(k.shape), list(v.shape)))
+    if D not in _HEAD_DIMS:
+        raise ValueError("a head dim of %d: %s are supported" % (D, _HEAD_DIMS))
+    if k.shape[2] == 0 or H == 0 or H % k.shape[2]:
+        raise ValueError("%d query heads over %d key heads" % (H, k.shape[2]))
+    if max(Lq, k.shape[1]) >= 1 << 22 or B * H >= 1 << 30:
+        raise ValueError("%d queries and %d keys of %d heads are too many" % (Lq, k.shape[1], B * H))
+    for t, name in ((q_lens, "q_lens"), (kv_lens, "kv_lens")):
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):
+            raise ValueError("%s must be a contiguous int32 [%d], got %s %s" % (name, B, t.dtype, list(t.shape)))
+    window, sinks = 0 if window is None else _count(window, "window", 1), _count(sinks, "sinks")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be a finite number, got %r" % scale)
+    return BandAttention.call(q, k, v, q_lens, kv_lens, window, sinks, 1 if causal else 0, scale)

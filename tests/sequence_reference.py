@@ -87,3 +87,52 @@ def select(weight, n, budget, sinks, recent):
     number = ~np.isnan(weight[middle])   # (every number before every NaN)
     best = middle[np.lexsort((middle, -key, ~number))[: budget - sinks - recent]]
     return np.sort(np.concatenate([np.arange(sinks), best, np.arange(n - recent, n)])).astype(np.int64)
+
+
+def band_attention(q, k, v, window, sinks, causal, scale=None, q_lens=None, kv_lens=None, do=None):
+    """-> dict of out (and dq, dk, dv) and of their bounds before the last rounding, arrays [B, L, heads, hd]"""
+    dtype = q.dtype
+    q, k, v, do = (f64(t) if t is not None else None for t in (q, k, v, do))
+    B, Lq, H, D = q.shape
+    Lk, kv = k.shape[1], k.shape[2]
+    G, scale = H // kv, (D ** -0.5 if scale is None else scale)
+    names = ("out",) if do is None else ("out", "dq", "dk", "dv")
+    shapes = dict(out=q.shape, dq=q.shape, dk=k.shape, dv=k.shape)
+    val, err = ({x: np.zeros(shapes[x]) for x in names} for _ in range(2))
+    h = 0.0 if dtype == torch.float32 else half_step(dtype)   # the rounding of weights and of score gradients to the type
+    for b in range(B):
+        m = Lq if q_lens is None else min(max(int(q_lens[b]), 0), Lq)
+        n = Lk if kv_lens is None else min(max(int(kv_lens[b]), 0), Lk)
+        if not m or not n:
+            continue
+        see = visible(m, n, window, sinks, causal)
+        for i in range(H):
+            qq, kk, vv = q[b, :m, i], k[b, :n, i // G], v[b, :n, i // G]
+            p = softmax_rows(qq @ kk.T * scale, see)
+            o = p @ vv
+            # a score is off by (D + 8) u of its absolute products, a weight by twice the row's worst of that (numerator and
+            # normaliser), plus exp2 and log2, the sums over n and the maximum carried: relatively to the weight
+            worst = np.where(see, np.abs(qq) @ np.abs(kk).T, 0.0).max(1, keepdims=True) * abs(scale)
+            rel = 2 * (D + 8) * U * worst + (n / 16 + 64) * U
+            val["out"][b, :m, i] = o
+            err["out"][b, :m, i] = p * (rel + h) @ np.abs(vv)
+            if dtype == torch.float16:   # below 2^-14 its steps are 2^-24: weights relative to the row's largest
+                err["out"][b, :m, i] += 2.0 ** -25 * see @ np.abs(vv)
+            if do is None:
+                continue
+            g = do[b, :m, i]
+            dp, delta = g @ vv.T, (g * o).sum(1, keepdims=True)
+            ds = p * (dp - delta)
+            # delta comes from the output as it was stored (half a step of the type, 32-bit sums on top)
+            e_delta = (np.abs(g) * (half_step(dtype) * np.abs(o) + err["out"][b, :m, i] + (D + 2) * U * np.abs(o))).sum(1, keepdims=True)
+            e_dp = (D + 2) * U * (np.abs(g) @ np.abs(vv).T)
+            e_ds = np.abs(ds) * (rel + h + 4 * U) + p * (1 + rel) * (e_dp + e_delta)
+            if dtype == torch.float16:   # ... and score gradients are carried up to 2^15, weights up to 2^10
+                e_ds = e_ds + see * 2.0 ** -38 * np.abs(ds).max()
+            val["dq"][b, :m, i] = scale * ds @ kk
+            err["dq"][b, :m, i] = abs(scale) * ((e_ds + (n / 16 + 8) * U * np.abs(ds)) @ np.abs(kk))
+            val["dk"][b, :n, i // G] += scale * ds.T @ qq
+            err["dk"][b, :n, i // G] += abs(scale) * ((e_ds + (m / 16 + 64 + 8 * G) * U * np.abs(ds)).T @ np.abs(qq))
+            val["dv"][b, :n, i // G] += p.T @ g
+            err["dv"][b, :n, i // G] += (p * (rel + h + (m / 16 + 64 + 8 * G) * U) + (2.0 ** -35 * see if dtype == torch.float16 else 0.0)).T @ np.abs(g)
+    return val, err

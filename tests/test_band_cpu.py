@@ -1,0 +1,69 @@
+"""Refusals of band attention, at the Python entry point and at the C boundary."""
+import ctypes
+
+import pytest
+import torch
+
+from interactron_amd import _lib, hipops
+
+BF16 = torch.bfloat16
+
+
+def qkv(B=2, Lq=5, Lk=7, H=4, kv=2, D=64, dtype=BF16):
+    return torch.zeros(B, Lq, H, D, dtype=dtype), torch.zeros(B, Lk, kv, D, dtype=dtype), torch.zeros(B, Lk, kv, D, dtype=dtype)
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(_lib.HipLibraryError, match="GPU"):
+        hipops.band_attention(*qkv())
+
+
+@pytest.mark.parametrize("shape, how, words", [
+    (dict(D=48), {}, "head dim of 48"), (dict(H=3), {}, "3 query heads"), (dict(kv=0), {}, "key heads"), (dict(dtype=torch.float64), {}, "q must be"),
+    ({}, dict(window=0), "window"), ({}, dict(window=-3), "window"), ({}, dict(window=1.5), "window"), ({}, dict(window=1 << 30), "window"),
+    ({}, dict(sinks=-1), "sinks"), ({}, dict(sinks=None), "sinks"), ({}, dict(scale=float("nan")), "scale"), ({}, dict(scale=float("inf")), "scale"),
+    ({}, dict(q_lens=torch.zeros(2)), "q_lens"), ({}, dict(kv_lens=torch.zeros(3, dtype=torch.int32)), "kv_lens"),
+    ({}, dict(kv_lens=torch.zeros(4, dtype=torch.int32)[::2]), "kv_lens"), ({}, dict(q_lens=torch.zeros(2, dtype=torch.int64)), "q_lens"),
+])
+def test_wrong_arguments_are_refused(shape, how, words):
+    with pytest.raises(ValueError, match=words):
+        hipops.band_attention(*qkv(**shape), **how)
+
+
+@pytest.mark.parametrize("change", [lambda q, k, v: (q[0], k, v), lambda q, k, v: (q, k.float(), v), lambda q, k, v: (q, k, v[:, :3]),
+                                    lambda q, k, v: (q[:1], k, v), lambda q, k, v: (q[..., :32], k, v), lambda q, k, v: (q, k[:, :, :1], v)])
+def test_tensors_that_do_not_fit_are_refused(change):
+    with pytest.raises(ValueError):
+        hipops.band_attention(*change(*qkv()))
+
+
+def c_band(**change):
+    """A description whose pointers are never followed"""
+    f = dict(q=4096, k=4096, v=4096, q_sb=1280, q_sl=256, q_sh=64, k_sb=896, k_sl=128, k_sh=64, v_sb=896, v_sl=128, v_sh=64, q_lens=None, kv_lens=None,
+             dtype=1, batch=2, Lq=5, Lk=7, heads=4, kv_heads=2, hd=64, window=0, sinks=0, causal=1, scale=0.125)
+    f.update(change)
+    return hipops.band._BandC(*[f[n] for n, _ in hipops.band._BandC._fields_])
+
+
+@pytest.mark.parametrize("change", [dict(q=None), dict(k=None), dict(v=4100), dict(dtype=3), dict(hd=80), dict(batch=0), dict(Lq=0), dict(Lk=0), dict(Lq=1 << 22),
+                                    dict(heads=3), dict(kv_heads=0), dict(heads=0), dict(window=-1), dict(sinks=-1), dict(scale=float("nan")),
+                                    dict(scale=float("inf")), dict(q_sl=252), dict(v_sh=33), dict(batch=1 << 29)], ids=str)
+def test_c_entries_refuse_a_bad_description(change):
+    L, c, n = _lib.load(), c_band(**change), ctypes.c_size_t(0)
+    for rc in (L.ix_band_attn_fwd(ctypes.byref(c), 4096, 4096, None), L.ix_workspace_bytes_band_attn_bwd(ctypes.byref(c), ctypes.byref(n)),
+               L.ix_band_attn_bwd(ctypes.byref(c), 4096, 4096, 4096, 1280, 256, 64, 4096, 4096, 4096, 4096, 1 << 30, None)):
+        assert rc == -1 and L.ix_last_error()
+
+
+def test_c_entries_refuse_bad_buffers():
+    L, c, n = _lib.load(), c_band(), ctypes.c_size_t(0)
+    ref = ctypes.byref(c)
+    assert L.ix_band_attn_fwd(ref, None, None, None) == -1 and L.ix_band_attn_fwd(ref, 4104, None, None) == -1
+    assert L.ix_workspace_bytes_band_attn_bwd(ref, ctypes.byref(n)) == 0 and n.value >= 2 * 4 * 128 * 4
+    good = [ref, 4096, 4096, 4096, 1280, 256, 64, 4096, 4096, 4096, 4096, n.value, None]
+    for place, value, code in ((1, None, -1), (2, None, -1), (3, 4104, -1), (5, 100, -1), (7, None, -1), (8, 4104, -1), (10, None, -3), (10, 4100, -3), (11, n.value - 1, -3)):
+        args = list(good)
+        args[place] = value
+        assert L.ix_band_attn_bwd(*args) == code, (place, L.ix_last_error())
+    p = ctypes.c_int64(0)
+    assert L.ix_band_attn_lse_pitch(0, ctypes.byref(p)) == -1 and L.ix_band_attn_lse_pitch(129, ctypes.byref(p)) == 0 and p.value == 256
