@@ -538,9 +538,9 @@ int ix_adam_step_f32(float* p, float* g, float* m, float* v, int64_t n, float lr
  * sh; rows dense and on 16 bytes); query head h reads key head h / (heads / kv_heads).  dtype 0 f32, 1 bf16, 2 fp16; hd 32, 64, 128.
  * q_lens, kv_lens int32 [batch] (null: Lq, Lk): rows behind them are never read and come back as zeros.  A query that sees nothing
  * gives zeros and has no gradient.  Keys and values that a query does not see have to be finite where they lie inside the lengths.
- *   ix_band_attn_fwd : out [batch][Lq][heads][hd] dense; lse (may be null) f32 [batch][heads][pitch], base 2, for the gradients;
- *                      pitch from ix_band_attn_lse_pitch
- *   ix_band_attn_bwd : dq, dk, dv (dense, like q, k, v) from out, lse and d_out [batch][Lq][heads][hd] by strides g_*; sums in f32,
+ *   ix_band_attn_fwd : out [batch][Lq][heads][hd] dense; for the gradients (may be null) lse f32 [batch][heads][pitch], base 2 (pitch
+ *                      from ix_band_attn_lse_pitch), and rest like out: what its rounding to 16 bits took away (not with f32)
+ *   ix_band_attn_bwd : dq, dk, dv (dense, like q, k, v) from out, rest, lse and d_out [batch][Lq][heads][hd] by strides g_*; sums in f32,
  *                      in a fixed order (no atomics); workspace of ix_workspace_bytes_band_attn_bwd bytes, 16-byte aligned */
 struct ix_band {
     const void *q, *k, *v;
@@ -549,11 +549,11 @@ struct ix_band {
     int dtype, batch, Lq, Lk, heads, kv_heads, hd, window, sinks, causal;
     float scale;
 };
-int ix_band_attn_fwd(const struct ix_band* band_host, void* out, float* lse, ix_stream_t stream);
+int ix_band_attn_fwd(const struct ix_band* band_host, void* out, float* lse, void* rest, ix_stream_t stream);
 int ix_band_attn_lse_pitch(int Lq, int64_t* out_host);
 int ix_workspace_bytes_band_attn_bwd(const struct ix_band* band_host, size_t* out_host);
-int ix_band_attn_bwd(const struct ix_band* band_host, const void* out, const float* lse, const void* d_out, int64_t g_sb, int64_t g_sl,
-                     int64_t g_sh, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, ix_stream_t stream);
+int ix_band_attn_bwd(const struct ix_band* band_host, const void* out, const void* rest, const float* lse, const void* d_out, int64_t g_sb,
+                     int64_t g_sl, int64_t g_sh, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, ix_stream_t stream);
 
 /* ---- A paged cache of keys and values (csrc/cache.hip): acting on a rollout that grows token by token --------------------------------
  * The reference runs its fusion transformer over the whole sequence again for every new frame (models/transformer.py:49-60,

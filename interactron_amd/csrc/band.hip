@@ -5,7 +5,7 @@
 // q, do, out, dq [B][Lq][H][D], k, v, dk, dv [B][Lk][kv][D]; query head h reads key head h / (H / kv), so dk, dv sum over the group.
 // Rows behind a sequence's lengths are not read (they may hold anything) and come back as zeros; a query that sees nothing gives zeros.
 //
-// Three kernels, all of one shape: a workgroup of four waves OWNS rows (queries: forward and dq; keys: dk / dv) that live in registers as
+// Three products' loops, all of one shape: a workgroup of four waves OWNS rows (queries: forward and dq; keys: dk / dv) that live in registers as
 // the matrix instructions' B operands, and STREAMS tiles of the other side through LDS.  A tile of products comes out of the matrix
 // instructions with owner rows in the lanes' columns and streamed rows in the registers: softmax statistics and the row constants of the
 // gradients are per lane, and the accumulator of one product is, rounded, the B operand of the next (contracting over streamed rows) --
@@ -19,6 +19,12 @@ namespace {
 
 constexpr int kBlock = 256, kWaves = 4;
 constexpr int kFar = 1 << 30;   // an unlimited band (lengths stay below 2^28)
+
+// owner rows of a wave: two blocks of 16 with 16-bit operands, one with f32 (twice the registers an element)
+constexpr int owner_blocks(int dt) { return dt == 0 ? 1 : 2; }
+constexpr int owner_rows(int dt) { return 16 * owner_blocks(dt) * kWaves; }
+constexpr int key_tile(int dt) { return dt == 0 ? 32 : 64; }
+constexpr int query_tile(int dt, int hd) { return dt == 0 || hd == 128 ? 32 : 64; }
 
 // ---- the LDS image of a tile of rows ------------------------------------------------------------------------------------------------
 // 32-byte pairs of a row change places by the row's number, so that eight neighbouring rows' pieces lie in different banks for both ways
@@ -88,13 +94,13 @@ template <int DT, int D, int ROWS> struct Stage {
 };
 
 struct BandArgs {
-    const unsigned char *q, *k, *v, *go, *o;
+    const unsigned char *q, *k, *v, *go, *o, *o_rest;
     int64_t qb, ql, qh, kb, kl, kh, vb, vl, vh, gb, gl, gh;   // bytes
-    unsigned char *out, *dq, *dk, *dv;                        // dense
+    unsigned char *out, *rest, *dq, *dk, *dv;                 // dense; rest: what rounding the output to 16 bits took away, in 16 bits
     float *lse, *delta, *part;                                // [B][H][Lp] base-2 normalisers (+inf: nothing visible) and delta; partial sums
     const int *q_lens, *kv_lens;
     int B, Lq, Lk, Lp, H, kv, left, right, sinks, causal;
-    int wide_blocks, wide_splits, splits;                     // dk / dv: see the host side
+    int wide_blocks, wide_splits, splits, key_groups;         // dk / dv: see the host side; workgroups of theirs
     float c2, scale;                                          // |scale| log2(e), scale
     unsigned flip;                                            // sign bits of a fragment's register where scale < 0
     __device__ __forceinline__ int m(int b) const { return q_lens ? min(max(q_lens[b], 0), Lq) : Lq; }
@@ -308,24 +314,69 @@ __global__ __launch_bounds__(kBlock, 2) void band_fwd_kernel(BandArgs a) {
         const float inv = 1.f / total;
         if (a.lse && g == 0 && i < a.Lp) a.lse[(int64_t)bh * a.Lp + i] = none ? INFINITY : top[nb] + __log2f(total);
         if (i >= a.Lq) continue;
-        unsigned char* dst = a.out + (((int64_t)b * a.Lq + i) * a.H + h) * I::ROW;
+        const int64_t at = (((int64_t)b * a.Lq + i) * a.H + h) * I::ROW;
 #pragma unroll
-        for (int db = 0; db < I::DB; ++db) store4<DT>(dst + (16 * db + 4 * g) * I::EB, none ? f32x4{0.f, 0.f, 0.f, 0.f} : o[nb][db] * inv);
+        for (int db = 0; db < I::DB; ++db) {
+            const f32x4 x = none ? f32x4{0.f, 0.f, 0.f, 0.f} : o[nb][db] * inv;
+            store4<DT>(a.out + at + (16 * db + 4 * g) * I::EB, x);
+            if constexpr (DT != 0) {
+                if (a.rest) {
+                    f32x4 y;
+#pragma unroll
+                    for (int r = 0; r < 4; r += 2) {
+                        const unsigned w = seq_pack<DT>(x[r], x[r + 1]);
+                        y[r] = x[r] - seq_lo<DT>(w);
+                        y[r + 1] = x[r + 1] - seq_hi<DT>(w);
+                    }
+                    store4<DT>(a.rest + at + (16 * db + 4 * g) * I::EB, y);
+                }
+            }
+        }
     }
 }
 
 // ====================================================================================================================================
 // gradients
 // ====================================================================================================================================
-// dq, and delta for the other kernel: query-owning, streams k (both ways) and v (rows).  Tiles are taken 32 keys at a time.
+// delta_i = do_i o_i, a row by the lanes that hold 16 bytes of it each.  16-bit: o is the stored output and the rest its rounding took, so
+// that delta -- which is subtracted from every do_i v_j of the row -- is as good as from the 32-bit output.
+template <int DT, int D>
+__global__ __launch_bounds__(kBlock) void band_delta_kernel(BandArgs a) {
+    constexpr int EB = SeqT<DT>::bytes, LANES = D * EB / 16;
+    const int64_t row = ((int64_t)blockIdx.x * kBlock + threadIdx.x) / LANES;   // (batch, query, head)
+    const int c = threadIdx.x % LANES, h = (int)(row % a.H);
+    const int64_t bi = row / a.H;
+    const int i = (int)(bi % a.Lp), b = (int)(bi / a.Lp);
+    if (b >= a.B) return;   // (whole rows: the lanes of a row leave together)
+    float d = 0.f;
+    if (i < a.m(b)) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(a.go + b * a.gb + i * a.gl + h * a.gh + 16 * c);
+        const int64_t at = (((int64_t)b * a.Lq + i) * a.H + h) * (D * EB) + 16 * c;
+        const u32x4 y = *reinterpret_cast<const u32x4*>(a.o + at);
+        if constexpr (DT == 0) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) d += __uint_as_float(x[w]) * __uint_as_float(y[w]);
+        } else {
+            const u32x4 z = *reinterpret_cast<const u32x4*>(a.o_rest + at);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                d += seq_lo<DT>(x[w]) * (seq_lo<DT>(y[w]) + seq_lo<DT>(z[w])) + seq_hi<DT>(x[w]) * (seq_hi<DT>(y[w]) + seq_hi<DT>(z[w]));
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) d += __shfl_xor(d, o, 64);
+    if (c == 0) a.delta[((int64_t)b * a.H + h) * a.Lp + i] = d;
+}
+
+// dq: query-owning, streams k (both ways) and v (rows).  Tiles are taken 32 keys at a time.
 template <int DT, int D, int NB, int TB>
-__global__ __launch_bounds__(kBlock, D == 128 && DT != 0 ? 1 : 2) void band_dq_kernel(BandArgs a) {
+__device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, int group) {
     typedef Img<DT, D> I;
     constexpr int ROWS = 16 * NB * kWaves, BYTES = TB * I::ROW;
-    __shared__ __attribute__((aligned(256))) unsigned char lds[2][2][BYTES];
+    auto lds = reinterpret_cast<unsigned char (*)[2][BYTES]>(mem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
-    const int bh = spread_heads(blockIdx.x, a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.kv);
-    const int blk = a.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y, i0 = blk * ROWS;
+    const int bh = spread_heads(group % (a.B * a.H), a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.kv);
+    const int blocks = (a.Lq + ROWS - 1) / ROWS, y = group / (a.B * a.H), i0 = (a.causal ? blocks - 1 - y : y) * ROWS;
     const int m = a.m(b), n = a.n(b), shift = n - m, iw = i0 + wave * 16 * NB;
     f32x4 acc[NB][I::DB];
     float lse[NB], delta[NB], F[NB];
@@ -342,22 +393,12 @@ __global__ __launch_bounds__(kBlock, D == 128 && DT != 0 ? 1 : 2) void band_dq_k
         Frag<DT> qf[NB][I::KS], gf[NB][I::KS];
         owner_frags<DT, D, NB>(qf, a.q + b * a.qb + h * a.qh, a.ql, iw, m, n16, g, a.flip);
         owner_frags<DT, D, NB>(gf, a.go + b * a.gb + h * a.gh, a.gl, iw, m, n16, g, 0u);
-        {
-            Frag<DT> of[NB][I::KS];
-            owner_frags<DT, D, NB>(of, a.o + ((int64_t)b * a.Lq * a.H + h) * I::ROW, (int64_t)a.H * I::ROW, iw, m, n16, g, 0u);
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                float d = 0.f;
-#pragma unroll
-                for (int ks = 0; ks < I::KS; ++ks)
-#pragma unroll
-                    for (int w = 0; w < SeqT<DT>::words; ++w) {
-                        if constexpr (DT == 0) d += __uint_as_float(gf[nb][ks].w[w]) * __uint_as_float(of[nb][ks].w[w]);
-                        else d += seq_lo<DT>(gf[nb][ks].w[w]) * seq_lo<DT>(of[nb][ks].w[w]) + seq_hi<DT>(gf[nb][ks].w[w]) * seq_hi<DT>(of[nb][ks].w[w]);
-                    }
-                delta[nb] = seq_sum_g(d);
-                const int i = iw + 16 * nb + n16;
-                if (i < m) lse[nb] = a.lse[(int64_t)bh * a.Lp + i];
+        for (int nb = 0; nb < NB; ++nb) {
+            const int i = iw + 16 * nb + n16;
+            if (i < m) {
+                lse[nb] = a.lse[(int64_t)bh * a.Lp + i];
+                delta[nb] = a.delta[(int64_t)bh * a.Lp + i];
             }
         }
         const unsigned char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
@@ -438,7 +479,6 @@ __global__ __launch_bounds__(kBlock, D == 128 && DT != 0 ? 1 : 2) void band_dq_k
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const int i = iw + 16 * nb + n16;
-        if (g == 0 && i < a.Lp) a.delta[(int64_t)bh * a.Lp + i] = delta[nb];
         if (i >= a.Lq) continue;
         const float f = DT == 2 ? a.scale / F[nb] : a.scale;
         unsigned char* dst = a.dq + (((int64_t)b * a.Lq + i) * a.H + h) * I::ROW;
@@ -462,14 +502,14 @@ struct KeyItem {
 };
 
 template <int DT, int D, int NB, int TB>
-__global__ __launch_bounds__(kBlock, D == 128 && DT != 0 ? 1 : 2) void band_dkv_kernel(BandArgs a) {
+__device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, int group) {
     typedef Img<DT, D> I;
     constexpr int ROWS = 16 * NB * kWaves, BYTES = TB * I::ROW;
-    __shared__ __attribute__((aligned(256))) unsigned char lds[2][2][BYTES];
-    __shared__ __attribute__((aligned(16))) float row_c[2][2][TB];   // lse, delta of the tile's queries
+    auto lds = reinterpret_cast<unsigned char (*)[2][BYTES]>(mem);
+    auto row_c = reinterpret_cast<float (*)[2][TB]>(mem + 4 * BYTES);   // lse, delta of the tile's queries
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
-    const int bk = spread_heads(blockIdx.x, a.B * a.kv), b = bk / a.kv, hk = bk % a.kv, G = a.H / a.kv;
-    const KeyItem it(a, blockIdx.y);
+    const int bk = spread_heads(group % (a.B * a.kv), a.B * a.kv), b = bk / a.kv, hk = bk % a.kv, G = a.H / a.kv, item = group / (a.B * a.kv);
+    const KeyItem it(a, item);
     const int m = a.m(b), n = a.n(b), shift = n - m, j0 = it.block * ROWS, jw = j0 + wave * 16 * NB;
     f32x4 ak[NB][I::DB], av[NB][I::DB];
     float F[NB];
@@ -592,7 +632,7 @@ __global__ __launch_bounds__(kBlock, D == 128 && DT != 0 ? 1 : 2) void band_dkv_
             for (int db = 0; db < I::DB; ++db) ak[nb][db] = av[nb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         if (it.splits > 1) {
-            float* dst = a.part + (((int64_t)bk * gridDim.y + blockIdx.y) * 2 * ROWS + row) * D;
+            float* dst = a.part + (((int64_t)bk * (a.key_groups / (a.B * a.kv)) + item) * 2 * ROWS + row) * D;
 #pragma unroll
             for (int db = 0; db < I::DB; ++db) {
                 *reinterpret_cast<f32x4*>(dst + 16 * db + 4 * g) = ak[nb][db] * fk;
@@ -607,6 +647,18 @@ __global__ __launch_bounds__(kBlock, D == 128 && DT != 0 ? 1 : 2) void band_dkv_
             }
         }
     }
+}
+
+// Both in one launch, the key blocks first: either alone would leave compute units empty at the sizes where time counts, and at its end.
+template <int DT, int D> constexpr int bwd_bytes() {
+    constexpr int q = 4 * key_tile(DT) * Img<DT, D>::ROW, k = 4 * query_tile(DT, D) * Img<DT, D>::ROW + 16 * query_tile(DT, D);
+    return q > k ? q : k;
+}
+template <int DT, int D, int NB>
+__global__ __launch_bounds__(kBlock, D == 128 && DT != 0 ? 1 : 2) void band_bwd_kernel(BandArgs a) {
+    __shared__ __attribute__((aligned(256))) unsigned char mem[bwd_bytes<DT, D>()];
+    if ((int)blockIdx.x < a.key_groups) band_dkv<DT, D, NB, query_tile(DT, D)>(a, mem, blockIdx.x);
+    else band_dq<DT, D, NB, key_tile(DT)>(a, mem, blockIdx.x - a.key_groups);
 }
 
 // dk, dv of the blocks that were cut into splits: the partial sums in split order, four values a thread
@@ -631,12 +683,6 @@ __global__ __launch_bounds__(kBlock) void band_sum_kernel(BandArgs a, int items,
 // ====================================================================================================================================
 // host side
 // ====================================================================================================================================
-// owner rows of a wave: two blocks of 16 with 16-bit operands, one with f32 (twice the registers an element)
-constexpr int owner_blocks(int dt) { return dt == 0 ? 1 : 2; }
-constexpr int owner_rows(int dt) { return 16 * owner_blocks(dt) * kWaves; }
-constexpr int key_tile(int dt) { return dt == 0 ? 32 : 64; }
-constexpr int query_tile(int dt, int hd) { return dt == 0 || hd == 128 ? 32 : 64; }
-
 struct KeyPlan { int blocks, wide, wide_splits, splits, items; };
 
 // Splits of dk / dv.  A block of keys streams the queries of its band; a block with some of the first `sinks` keys streams all of them, and
@@ -711,11 +757,12 @@ int band_of(BandArgs& a, const ix_band* s, const char* who) {
 #define BAND_HD(CALL, DT) { if (s->hd == 32) CALL(DT, 32); else if (s->hd == 64) CALL(DT, 64); else CALL(DT, 128); }
 #define BAND_GO(CALL) { if (s->dtype == 0) BAND_HD(CALL, 0) else if (s->dtype == 1) BAND_HD(CALL, 1) else BAND_HD(CALL, 2) }
 
-extern "C" int ix_band_attn_fwd(const struct ix_band* s, void* out, float* lse, hipStream_t stream) {
+extern "C" int ix_band_attn_fwd(const struct ix_band* s, void* out, float* lse, void* rest, hipStream_t stream) {
     BandArgs a;
     if (int rc = band_of(a, s, "ix_band_attn_fwd")) return rc;
-    IX_CHECK_ARG(out && ix_al16(out), "ix_band_attn_fwd: null or unaligned output");
+    IX_CHECK_ARG(out && ix_al16(out) && ix_al16(rest), "ix_band_attn_fwd: null or unaligned output");
     a.out = static_cast<unsigned char*>(out);
+    a.rest = s->dtype ? static_cast<unsigned char*>(rest) : nullptr;
     a.lse = lse;
     const dim3 grid(a.B * a.H, (a.Lq + owner_rows(s->dtype) - 1) / owner_rows(s->dtype));
 #define BAND_FWD(DT, D) band_fwd_kernel<DT, D, owner_blocks(DT), key_tile(DT)><<<grid, kBlock, 0, stream>>>(a)
@@ -740,22 +787,22 @@ extern "C" int ix_workspace_bytes_band_attn_bwd(const struct ix_band* s, size_t*
     return IX_OK;
 }
 
-extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const float* lse, const void* d_out, int64_t g_sb, int64_t g_sl, int64_t g_sh,
-                                void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const void* rest, const float* lse, const void* d_out, int64_t g_sb, int64_t g_sl,
+                                int64_t g_sh, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     BandArgs a;
     if (int rc = band_of(a, s, "ix_band_attn_bwd")) return rc;
     const int64_t eb = s->dtype == 0 ? 4 : 2;
-    IX_CHECK_ARG(out && lse && d_out && dq && dk && dv, "ix_band_attn_bwd: null pointer");
-    IX_CHECK_ARG(ix_al16(out) && ix_al16(d_out) && ix_al16(dq) && ix_al16(dk) && ix_al16(dv), "ix_band_attn_bwd: unaligned pointer");
+    IX_CHECK_ARG(out && (rest || s->dtype == 0) && lse && d_out && dq && dk && dv, "ix_band_attn_bwd: null pointer");
+    IX_CHECK_ARG(ix_al16(out) && ix_al16(rest) && ix_al16(d_out) && ix_al16(dq) && ix_al16(dk) && ix_al16(dv), "ix_band_attn_bwd: unaligned pointer");
     for (int64_t x : {g_sb, g_sl, g_sh}) IX_CHECK_ARG(x * eb % 16 == 0, "ix_band_attn_bwd: rows that do not start on 16 bytes");
     const KeyPlan r = key_plan(s);
-    const size_t need = (size_t)a.B * a.H * a.Lp * 4 + part_bytes(s, r);
+    const size_t parts = part_bytes(s, r), need = (size_t)a.B * a.H * a.Lp * 4 + parts;
     if (!workspace || workspace_bytes < need || !ix_al16(workspace)) {
         ix_set_error("ix_band_attn_bwd: workspace of %zu bytes (16-byte aligned), %zu needed", workspace ? workspace_bytes : (size_t)0, need);
         return IX_ERR_WORKSPACE;
     }
-    IX_CHECK_ARG(r.items <= 65535, "ix_band_attn_bwd: too many keys for one launch");
     a.o = static_cast<const unsigned char*>(out);
+    a.o_rest = static_cast<const unsigned char*>(rest);
     a.go = static_cast<const unsigned char*>(d_out);
     a.gb = g_sb * eb; a.gl = g_sl * eb; a.gh = g_sh * eb;
     a.lse = const_cast<float*>(lse);
@@ -767,15 +814,20 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
     a.wide_blocks = r.wide;
     a.wide_splits = r.wide_splits;
     a.splits = r.splits;
-    const dim3 qgrid(a.B * a.H, (a.Lq + owner_rows(s->dtype) - 1) / owner_rows(s->dtype)), kgrid(a.B * a.kv, r.items);
-#define BAND_DQ(DT, D) band_dq_kernel<DT, D, owner_blocks(DT), key_tile(DT)><<<qgrid, kBlock, 0, stream>>>(a)
-    BAND_GO(BAND_DQ)
-    IX_CHECK_LAUNCH("ix_band_attn_bwd (dq)");
-#define BAND_DKV(DT, D) band_dkv_kernel<DT, D, owner_blocks(DT), query_tile(DT, D)><<<kgrid, kBlock, 0, stream>>>(a)
-    BAND_GO(BAND_DKV)
-    IX_CHECK_LAUNCH("ix_band_attn_bwd (dk, dv)");
-    if (part_bytes(s, r)) {
+    const int rows = owner_rows(s->dtype);
+    const int64_t key_groups = (int64_t)a.B * a.kv * r.items, groups = key_groups + (int64_t)a.B * a.H * ((a.Lq + rows - 1) / rows);
+    const int64_t delta_groups = ((int64_t)a.B * a.H * a.Lp * (s->hd * eb / 16) + kBlock - 1) / kBlock;
+    IX_CHECK_ARG(groups < (1ll << 31) && delta_groups < (1ll << 31), "ix_band_attn_bwd: too many rows for one launch");
+    a.key_groups = (int)key_groups;
+#define BAND_DELTA(DT, D) band_delta_kernel<DT, D><<<(unsigned)delta_groups, kBlock, 0, stream>>>(a)
+    BAND_GO(BAND_DELTA)
+    IX_CHECK_LAUNCH("ix_band_attn_bwd (delta)");
+#define BAND_BWD(DT, D) band_bwd_kernel<DT, D, owner_blocks(DT)><<<(unsigned)groups, kBlock, 0, stream>>>(a)
+    BAND_GO(BAND_BWD)
+    IX_CHECK_LAUNCH("ix_band_attn_bwd");
+    if (parts) {
         const int blocks = r.splits > 1 ? r.blocks : r.wide;
+        IX_CHECK_ARG(blocks <= 65535, "ix_band_attn_bwd: too many keys for one launch");
         const dim3 sgrid(a.B * a.kv, blocks, 4);
 #define BAND_SUM(DT, D) band_sum_kernel<DT, D><<<sgrid, kBlock, 0, stream>>>(a, r.items, owner_rows(DT))
         BAND_GO(BAND_SUM)

@@ -10,7 +10,7 @@
 
 namespace {
 
-constexpr int kBlock = 256, kWaves = 4;
+constexpr int kBlock = 256;
 
 struct Cache {   // (the launch argument form of ix_paged_cache)
     unsigned char *k, *v;
@@ -126,12 +126,12 @@ template <int N> __device__ __forceinline__ void load_words(unsigned* w, const u
 //   into the pairs of keys that the matrix instruction wants.  P comes out of the scores' accumulator in exactly that key order.
 // P is carried as two 16-bit terms (hi + the rest), so that the sum keeps the precision of the f32 weights: the launch is bound by the
 // bytes of K and V, the second matrix instruction is free.
-template <int DT, int D>
-__global__ __launch_bounds__(kBlock, 2) void cache_attn_kernel(AttnArgs p) {
+template <int DT, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_kernel(AttnArgs p) {
     constexpr int KT = tile_keys<DT>(), NS = KT / 16, EB = SeqT<DT>::bytes, KSTEPS = D / 32, DB = D / 16;
     constexpr int VK = KT / 4, VW = DB * EB / 4;   // keys of V per lane, registers of one of them
-    __shared__ float lds_o[kWaves][16][D + 4];
-    __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
+    __shared__ float lds_o[WAVES][16][D + 4];
+    __shared__ float lds_m[WAVES][16], lds_l[WAVES][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
     const int split = blockIdx.x, b = blockIdx.z, h = blockIdx.y % p.c.kv, qt = blockIdx.y / p.c.kv;
     const int rows = min(16, p.group - 16 * qt), head0 = h * p.group + 16 * qt;   // this workgroup's query heads
@@ -154,11 +154,12 @@ __global__ __launch_bounds__(kBlock, 2) void cache_attn_kernel(AttnArgs p) {
     const int page_mask = (1 << p.c.shift) - 1;
     Frag<DT> kf[NS][KSTEPS];
     unsigned vf[VK][VW];
-    unsigned bad = 0;   // bit s: sub-tile s lies in no page of the pool
-    auto load = [&](int t) {
+    // a tile's page rows are looked up while the tile in front of it is requested, its keys and values while that one is worked on
+    int64_t row[NS];
+    unsigned bad = 0, bad_now = 0;   // bit s: sub-tile s lies in no page of the pool
+    auto find = [&](int t) {
         const int j0 = tl.base(t, KT);
         bad = 0;
-        int64_t row[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const int j = j0 + 16 * s;
@@ -166,18 +167,28 @@ __global__ __launch_bounds__(kBlock, 2) void cache_attn_kernel(AttnArgs p) {
             if (r < 0) bad |= 1u << s;
             row[s] = r < 0 ? 0 : r + (j & page_mask);   // (row 0 is in the pool: its values are masked)
         }
+    };
+    auto load = [&](int t) {
+        int64_t at[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) at[s] = row[s];
+        bad_now = bad;
+        if (t + WAVES < t1) find(t + WAVES);
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const unsigned char* kr = p.c.k + (row[s] + n) * (D * EB) + g * (8 * EB);
+            const unsigned char* kr = p.c.k + (at[s] + n) * (D * EB) + g * (8 * EB);
 #pragma unroll
             for (int ks = 0; ks < KSTEPS; ++ks) load_words<SeqT<DT>::words>(kf[s][ks].w, kr + ks * (32 * EB));
         }
 #pragma unroll
-        for (int i = 0; i < VK; ++i) load_words<VW>(vf[i], p.c.v + (row[i / 4] + 4 * g + i % 4) * (D * EB) + n * (DB * EB));
+        for (int i = 0; i < VK; ++i) load_words<VW>(vf[i], p.c.v + (at[i / 4] + 4 * g + i % 4) * (D * EB) + n * (DB * EB));
     };
     int t = t0 + wave;
-    if (t < t1) load(t);
-    for (; t < t1; t += kWaves) {
+    if (t < t1) {
+        find(t);
+        load(t);
+    }
+    for (; t < t1; t += WAVES) {
         const int j0 = tl.base(t, KT);
         f32x4 x[NS];
 #pragma unroll
@@ -192,18 +203,18 @@ __global__ __launch_bounds__(kBlock, 2) void cache_attn_kernel(AttnArgs p) {
         for (int i = 0; i < VK; ++i)
 #pragma unroll
             for (int w = 0; w < VW; ++w) vc[i][w] = vf[i][w];
-        if (bad || !tl.whole(j0, KT)) {   // masked keys: no score, and zeros for values (what lies there may be anything)
+        if (bad_now || !tl.whole(j0, KT)) {   // masked keys: no score, and zeros for values (what lies there may be anything)
 #pragma unroll
             for (int i = 0; i < VK; ++i) {
                 const int s = i / 4, j = j0 + 16 * s + 4 * g + i % 4;
                 // (selects, no branch: ROCm 7.2's compiler lost the first element's store of a short-circuit form of this)
-                const bool see = tl.sees(j) & !(bad >> s & 1);
+                const bool see = tl.sees(j) & !(bad_now >> s & 1);
                 x[s][i % 4] = see ? x[s][i % 4] : -INFINITY;
 #pragma unroll
                 for (int w = 0; w < VW; ++w) vc[i][w] = see ? vc[i][w] : 0;
             }
         }
-        if (t + kWaves < t1) load(t + kWaves);
+        if (t + WAVES < t1) load(t + WAVES);
         if (p.accumulate && n < rows) {
             float* dst = p.logits + (((int64_t)b * p.heads + head0 + n) * p.max_tiles + t) * KT + 4 * g;
 #pragma unroll
@@ -256,14 +267,14 @@ __global__ __launch_bounds__(kBlock, 2) void cache_attn_kernel(AttnArgs p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) lds_o[wave][n][(4 * g + r) * DB + db] = o[db][r];
     __syncthreads();
-    for (int i = tid; i < rows * D; i += kBlock) {
+    for (int i = tid; i < rows * D; i += 64 * WAVES) {
         const int q = i / D, d = i % D;
         float top = -INFINITY, sum = 0.f, acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, lds_m[w][q]);
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds_m[w][q]);
         const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float f = seq_exp2(lds_m[w][q] - ref);
             sum += f * lds_l[w][q];
             acc += f * lds_o[w][q][d];
@@ -280,20 +291,25 @@ __global__ __launch_bounds__(kBlock, 2) void cache_attn_kernel(AttnArgs p) {
 
 // Joins the splits of one query head; with `accumulate` further workgroups add the weights P_j of 1024 tile slots each, summed over the
 // query heads of the key head in their order, to the cache's accumulated weights.
+constexpr int kJoinSplits = 1024;   // split factors that are in LDS at a time
+
 template <int DT>
 __global__ __launch_bounds__(kBlock) void cache_join_kernel(AttnArgs p, int D, int out_blocks, int weight_blocks) {
-    constexpr int KT = tile_keys<DT>();
+    constexpr int KT = tile_keys<DT>(), WAVES = kBlock / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    __shared__ float red[kBlock], stat[2 * 64];
+    __shared__ float red[kBlock], stat[2 * 64], factor[kJoinSplits];
     // (maximum, 1 / sum) of query head `at` over its splits, by one wave
     auto stats = [&](int64_t at, int used) {
-        const float* ml = p.part_ml + at * p.splits * 2;
+        const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + at * p.splits;
         float top = -INFINITY, sum = 0.f;
-        for (int s = lane; s < used; s += 64) top = fmaxf(top, ml[2 * s]);
-        top = ix_wave_max(top);
-        const float ref = top == -INFINITY ? 0.f : top;
-        for (int s = lane; s < used; s += 64) sum += ml[2 * s + 1] * seq_exp2(ml[2 * s] - ref);
-        sum = ix_wave_sum(sum);
+        for (int s = lane; s < used; s += 64) {   // (rescaled as it goes: one pass)
+            const float2 x = ml[s];
+            const float up = fmaxf(top, x.x), ref = up == -INFINITY ? 0.f : up;
+            sum = sum * seq_exp2(top - ref) + x.y * seq_exp2(x.x - ref);
+            top = up;
+        }
+        const float all = ix_wave_max(top), ref = all == -INFINITY ? 0.f : all;
+        sum = ix_wave_sum(sum * seq_exp2(top - ref));
         return float2{ref, sum == 0.f ? 0.f : 1.f / sum};
     };
     if ((int)blockIdx.x < out_blocks) {
@@ -301,56 +317,72 @@ __global__ __launch_bounds__(kBlock) void cache_join_kernel(AttnArgs p, int D, i
         const int b = (int)(at / p.heads);
         const Tiles tl(p.c.len(b), p.window, p.sinks, KT, p.splits, p.least);
         const int used = tl.used();
-        const float2 st = stats(at, used);
+        const float2 st = stats(at, used);   // (every wave for itself)
         const int d = tid % D, part = tid / D, parts = kBlock / D;
         float acc = 0.f;
-        for (int s = part; s < used; s += parts) acc += p.part_o[(at * p.splits + s) * D + d] * seq_exp2(p.part_ml[(at * p.splits + s) * 2] - st.x);
+        for (int s0 = 0; s0 < used; s0 += kJoinSplits) {
+            const int here = min(kJoinSplits, used - s0);
+            __syncthreads();
+            for (int s = tid; s < here; s += kBlock) factor[s] = seq_exp2(p.part_ml[(at * p.splits + s0 + s) * 2] - st.x) * st.y;
+            __syncthreads();
+            const float* src = p.part_o + (at * p.splits + s0) * D + d;
+            int s = part;
+            for (; s + 7 * parts < here; s += 8 * parts) {   // eight loads in flight
+                float x[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) x[u] = src[(int64_t)(s + u * parts) * D];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) acc += x[u] * factor[s + u * parts];
+            }
+            for (; s < here; s += parts) acc += src[(int64_t)s * D] * factor[s];
+        }
         red[tid] = acc;
         __syncthreads();
         if (part == 0) {
             for (int k = 1; k < parts; ++k) acc += red[k * D + d];
-            seq_store1<DT>(p.out, at * D + d, acc * st.y);
+            seq_store1<DT>(p.out, at * D + d, acc);
         }
         return;
     }
     const int item = blockIdx.x - out_blocks, chunk = item % weight_blocks, h = (item / weight_blocks) % p.c.kv, b = item / weight_blocks / p.c.kv;
     const Tiles tl(p.c.len(b), p.window, p.sinks, KT, p.splits, p.least);
     if (chunk * 1024 >= tl.count * KT) return;
-    const int used = tl.used();
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const int used = tl.used(), i0 = chunk * 1024 + 4 * tid;   // four neighbouring slots (of one tile)
+    const bool live = i0 < tl.count * KT;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int q0 = 0; q0 < p.group; q0 += 64) {
         const int qn = min(64, p.group - q0);
         __syncthreads();
-        for (int q = wave; q < qn; q += kWaves) {
+        for (int q = wave; q < qn; q += WAVES) {
             const float2 st = stats((int64_t)b * p.heads + h * p.group + q0 + q, used);
             if (lane == 0) { stat[2 * q] = st.x; stat[2 * q + 1] = st.y; }
         }
         __syncthreads();
-        for (int q = 0; q < qn; ++q) {
-            const float* src = p.logits + ((int64_t)b * p.heads + h * p.group + q0 + q) * p.max_tiles * KT;
+        if (live) {
+            const float* src = p.logits + ((int64_t)b * p.heads + h * p.group + q0) * p.max_tiles * KT + i0;
+            for (int q = 0; q < qn; ++q) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(src + (int64_t)q * p.max_tiles * KT);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int i = chunk * 1024 + u * kBlock + tid;
-                if (i < tl.count * KT) acc[u] += seq_exp2(src[i] - stat[2 * q]) * stat[2 * q + 1];
+                for (int u = 0; u < 4; ++u) acc[u] += seq_exp2(x[u] - stat[2 * q]) * stat[2 * q + 1];
             }
         }
     }
+    if (!live) return;
+    const int j = tl.base(i0 / KT, KT) + i0 % KT;
+    float* dst = p.c.weight + ((int64_t)b * p.c.kv + h) * p.c.cap() + j;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int i = chunk * 1024 + u * kBlock + tid;
-        if (i >= tl.count * KT) continue;
-        const int j = tl.base(i / KT, KT) + i % KT;
-        if (tl.sees(j)) p.c.weight[((int64_t)b * p.c.kv + h) * p.c.cap() + j] += acc[u];
-    }
+    for (int u = 0; u < 4; ++u)
+        if (tl.sees(j + u)) dst[u] += acc[u];
 }
 
 // ====================================================================================================================================
 // select: the tokens that stay
 // ====================================================================================================================================
 // One workgroup of 16 waves per (sequence, key head).  The r-th largest weight of the middle is found digit by digit (four passes of
-// eight bits over keys whose unsigned order is the weights' order); then every wave counts its own stretch of tokens, the counts are
-// summed in wave order, and the wave writes its kept indexes with ballots: ascending, and of equal weights the lowest indexes.
-constexpr int kSelBlock = 1024, kSelWaves = 16;
+// eight bits over keys whose unsigned order is the weights' order).  Every wave has a stretch of tokens of its own, up to 1024 of them in
+// registers for all passes (longer stretches are read again); at the end it counts what stays of it, the counts are summed in wave order,
+// and it writes its kept indexes with ballots: ascending, and of equal weights the lowest indexes.
+constexpr int kSelBlock = 1024, kSelWaves = 16, kSelHeld = 16;
 
 __device__ __forceinline__ unsigned weight_key(float w) {
     if (w != w) return 0u;   // a NaN counts less than every number
@@ -373,17 +405,34 @@ __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, 
         return;
     }
     const int m0 = sinks, m1 = n - recent;   // (sinks + recent <= budget < n)
+    unsigned need = budget - sinks - recent;
+    const int span = m1 - m0, each = ((span + kSelWaves - 1) / kSelWaves + 63) / 64 * 64, w0 = m0 + wave * each, w1 = min(m1, w0 + each);
+    unsigned held[kSelHeld];
+    // the keys of this wave's tokens from `from` on, 64 a register; places behind its stretch hold no token
+    auto fetch = [&](int from) {
+#pragma unroll
+        for (int u = 0; u < kSelHeld; ++u) {
+            const int i = from + 64 * u + lane;
+            held[u] = i < w1 ? __float_as_uint(w[i]) : 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < kSelHeld; ++u) held[u] = weight_key(__uint_as_float(held[u]));
+    };
+    constexpr int kPart = 64 * kSelHeld;
+    const bool once = each <= kPart;
+    if (need && once) fetch(w0);
     for (int i = tid; i < sinks; i += kSelBlock) out[i] = i;
     for (int i = tid; i < recent; i += kSelBlock) out[budget - recent + i] = m1 + i;
-    unsigned need = budget - sinks - recent;
     if (need == 0) return;
     unsigned prefix = 0, mask = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
         for (int i = tid; i < kSelWaves * 256; i += kSelBlock) (&hist[0][0])[i] = 0;
         __syncthreads();
-        for (int i = m0 + tid; i < m1; i += kSelBlock) {
-            const unsigned u = weight_key(w[i]);
-            if ((u & mask) == prefix) atomicAdd(&hist[wave][(u >> shift) & 255], 1u);
+        for (int from = w0; from < w1; from += kPart) {
+            if (!once) fetch(from);
+#pragma unroll
+            for (int u = 0; u < kSelHeld; ++u)
+                if (from + 64 * u + lane < w1 && (held[u] & mask) == prefix) atomicAdd(&hist[wave][(held[u] >> shift) & 255], 1u);
         }
         __syncthreads();
         if (tid < 256) {
@@ -416,32 +465,35 @@ __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, 
         prefix |= pick[0] << shift;
         mask |= 255u << shift;
         need = pick[1];
-        __syncthreads();
     }
     // `prefix` is the smallest weight that stays, `need` of its equals stay with it
-    const int span = m1 - m0, each = ((span + kSelWaves - 1) / kSelWaves + 63) / 64 * 64, w0 = m0 + wave * each, w1 = min(m1, w0 + each);
     int a = 0, e = 0;
-    for (int i = w0 + lane; i < w1; i += 64) {
-        const unsigned u = weight_key(w[i]);
-        a += u > prefix;
-        e += u == prefix;
-    }
+    for (int from = w0; from < w1; from += kPart) {
+        if (!once) fetch(from);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); e += __shfl_xor(e, o, 64); }
+        for (int u = 0; u < kSelHeld; ++u) {
+            const bool in = from + 64 * u + lane < w1;
+            a += __popcll(__ballot(in && held[u] > prefix));
+            e += __popcll(__ballot(in && held[u] == prefix));
+        }
+    }
     if (lane == 0) { more[wave] = a; same[wave] = e; }
     __syncthreads();
     int at = sinks, eq = 0;
     for (int k = 0; k < wave; ++k) { at += more[k] + min(same[k], max(0, (int)need - eq)); eq += same[k]; }
     const unsigned long long below = (1ull << lane) - 1;
-    for (int i0 = w0; i0 < w1; i0 += 64) {
-        const int i = i0 + lane;
-        const unsigned u = i < w1 ? weight_key(w[i]) : 0;
-        const unsigned long long equal = __ballot(i < w1 && u == prefix);
-        const bool stay = i < w1 && (u > prefix || (u == prefix && eq + __popcll(equal & below) < (int)need));
-        const unsigned long long all = __ballot(stay);
-        if (stay) out[at + __popcll(all & below)] = i;
-        at += __popcll(all);
-        eq += __popcll(equal);
+    for (int from = w0; from < w1; from += kPart) {
+        if (!once) fetch(from);
+#pragma unroll
+        for (int u = 0; u < kSelHeld; ++u) {
+            const int i = from + 64 * u + lane;
+            const unsigned long long equal = __ballot(i < w1 && held[u] == prefix);
+            const bool stay = i < w1 && (held[u] > prefix || (held[u] == prefix && eq + __popcll(equal & below) < (int)need));
+            const unsigned long long all = __ballot(stay);
+            if (stay) out[at + __popcll(all & below)] = i;
+            at += __popcll(all);
+            eq += __popcll(equal);
+        }
     }
 }
 
@@ -449,70 +501,97 @@ __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, 
 // compact: kept rows to the front, in place
 // ====================================================================================================================================
 // Row i takes what row kept[i] >= i held.  A workgroup walks one column slice of K or V (or the weights) of one (sequence, head) in
-// ascending chunks: all rows of a chunk are in registers before the first of them is written, and no later chunk reads a row that an
-// earlier one has written, because kept[] ascends.  So the move needs no second copy of the cache, and the next chunk's loads fly while
-// this one is stored.
+// ascending chunks of 256 rows: all rows of a chunk are in registers before the first of them is written, and no later chunk reads a row
+// that an earlier one has written, because kept[] ascends and is nowhere below its own place.  So the move needs no second copy of the
+// cache, and the next chunk's rows are on their way while this one is stored, its places (kept index, two page look-ups) a chunk before
+// that, the kept indexes themselves another one.
 struct CompactArgs {
     Cache c;
     const int *kept, *left;
-    int budget, row_bytes, slice, slices;   // slice: bytes of a row that one workgroup moves
+    int budget, row_bytes, slices;   // slices of 16 LANES bytes in a row
 };
 
-constexpr int kMove = 8;   // rows per thread and chunk
+constexpr int kChunk = kBlock;   // rows
 
 __device__ __forceinline__ int64_t row_at(const Cache& c, int b, int h, int t) {
     const int64_t r = c.page_row(b, h, t);
     return r < 0 ? -1 : r + (t & ((1 << c.shift) - 1));
 }
 
+template <int LANES>   // threads of a row's slice
 __global__ __launch_bounds__(kBlock) void compact_kernel(CompactArgs p) {
+    constexpr int PER = kBlock / LANES;   // rows of one pass; LANES passes a chunk
+    __shared__ int64_t place[4][kChunk][2];
     const int b = blockIdx.z, h = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, cap = p.c.cap();
     const int n = min(max(p.left[b], 0), min(p.budget, cap));
     const int* kept = p.kept + ((int64_t)b * p.c.kv + h) * p.budget;
+    auto kept_at = [&](int i) { return i < n ? kept[i] : -1; };
     if (part == 2 * p.slices) {   // the weights, and the length
         if (h == 0 && tid == 0) p.c.lens[b] = n;
         if (!p.c.weight) return;
         float* w = p.c.weight + ((int64_t)b * p.c.kv + h) * cap;
-        for (int i0 = 0; i0 < n; i0 += kBlock * kMove) {
-            float x[kMove];
-            bool move[kMove];
+        for (int i0 = 0; i0 < n; i0 += kBlock * 8) {
+            float x[8];
+            bool move[8];
 #pragma unroll
-            for (int u = 0; u < kMove; ++u) {
-                const int i = i0 + u * kBlock + tid, from = i < n ? kept[i] : -1;
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + u * kBlock + tid, from = kept_at(i);
                 move[u] = from > i && from < cap;
                 x[u] = move[u] ? w[from] : 0.f;
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
 #pragma unroll
-            for (int u = 0; u < kMove; ++u)
+            for (int u = 0; u < 8; ++u)
                 if (move[u]) w[i0 + u * kBlock + tid] = x[u];
         }
         return;
     }
-    unsigned char* pool = part < p.slices ? p.c.k : p.c.v;
-    const int lanes = p.slice / 16, per = kBlock / lanes;   // threads of a row, rows of one pass
-    const int64_t col = (int64_t)(part % p.slices) * p.slice + (tid % lanes) * 16;
-    for (int i0 = 0; i0 < n; i0 += per * kMove) {
-        u32x4 x[kMove];
-        int64_t to[kMove];
-#pragma unroll
-        for (int u = 0; u < kMove; ++u) {
-            const int i = i0 + u * per + tid / lanes, from = i < n ? kept[i] : -1;
-            to[u] = -1;
-            x[u] = u32x4{0, 0, 0, 0};
-            if (from > i && from < cap) {
-                const int64_t src = row_at(p.c, b, h, from);
-                to[u] = row_at(p.c, b, h, i);
-                if (src < 0) to[u] = -1;
-                else x[u] = *reinterpret_cast<const u32x4*>(pool + src * p.row_bytes + col);
-            }
+    unsigned char* pool = (part < p.slices ? p.c.k : p.c.v) + (int64_t)(part % p.slices) * (16 * LANES) + (tid % LANES) * 16;
+    const int chunks = (n + kChunk - 1) / kChunk, r0 = tid / LANES;
+    auto find = [&](int c, int from, int64_t& src, int64_t& dst) {   // where row c kChunk + tid comes from and goes to
+        const int i = c * kChunk + tid;
+        src = dst = -1;
+        if (from > i && from < cap) {
+            src = row_at(p.c, b, h, from);
+            dst = row_at(p.c, b, h, i);
+            if (src < 0 || dst < 0) src = dst = -1;
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this thread's rows are in registers ...
-        __syncthreads();                                    // ... and so are everybody's
+    };
+    u32x4 x[LANES], y[LANES];
+    auto load = [&](int c, u32x4 (&r)[LANES]) {
 #pragma unroll
-        for (int u = 0; u < kMove; ++u)
-            if (to[u] >= 0) *reinterpret_cast<u32x4*>(pool + to[u] * p.row_bytes + col) = x[u];
+        for (int u = 0; u < LANES; ++u) {
+            const int64_t src = place[c & 3][u * PER + r0][0];
+            r[u] = src >= 0 ? *reinterpret_cast<const u32x4*>(pool + src * p.row_bytes) : u32x4{0, 0, 0, 0};
+        }
+    };
+    int64_t src, dst;
+    int next = kept_at(2 * kChunk + tid);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        find(c, kept_at(c * kChunk + tid), src, dst);
+        place[c][tid][0] = src;
+        place[c][tid][1] = dst;
+    }
+    __syncthreads();
+    load(0, x);
+    for (int c = 0; c < chunks; ++c) {
+        find(c + 2, next, src, dst);
+        next = kept_at((c + 3) * kChunk + tid);
+        if (c + 1 < chunks) load(c + 1, y);
+#pragma unroll
+        for (int u = 0; u < LANES; ++u) asm volatile("" : "+v"(x[u]));   // this thread's rows of the chunk are in registers ...
+        place[(c + 2) & 3][tid][0] = src;
+        place[(c + 2) & 3][tid][1] = dst;
+        __syncthreads();                                                  // ... and so are everybody's
+#pragma unroll
+        for (int u = 0; u < LANES; ++u) {
+            const int64_t to = place[c & 3][u * PER + r0][1];
+            if (to >= 0) *reinterpret_cast<u32x4*>(pool + to * p.row_bytes) = x[u];
+        }
+#pragma unroll
+        for (int u = 0; u < LANES; ++u) x[u] = y[u];
     }
 }
 
@@ -536,13 +615,14 @@ int cache_of(Cache& c, const ix_paged_cache* s, const char* who) {
 }
 
 struct Plan {   // of one attention launch
-    int max_tiles, splits, least, qtiles, kt;
+    int max_tiles, splits, least, qtiles, kt, waves;
     bool join;
     size_t o, ml, logits;   // floats
 };
 
-// Splits: enough workgroups to keep every compute unit supplied with loads (two of four waves each are resident per unit; several times
-// that many, so that sequences of different lengths even out), none with more than 512 keys while there are fewer than 4 096 of them.
+// Splits.  A cache of up to 32 tiles is one piece for eight waves: no join, one launch.  Longer ones are cut into about 1 024 workgroups of
+// four waves (two to four of them are resident on a compute unit), in pieces of at least one tile a wave, and of at most 512 keys where
+// several sequences of different lengths have to even out.
 Plan plan_of(const ix_paged_cache* s, int heads, int window, int sinks, int accumulate) {
     Plan r;
     r.kt = s->dtype == 0 ? 16 : 32;
@@ -557,12 +637,17 @@ Plan plan_of(const ix_paged_cache* s, int heads, int window, int sinks, int accu
     const int group = heads / s->kv_heads;
     r.qtiles = (group + 15) / 16;
     const int64_t rows = (int64_t)s->batch * s->kv_heads * r.qtiles;
-    const int64_t most = 512 / r.kt;
-    int64_t per = rows * seen / 2048;
-    r.least = kWaves;
-    if (per < r.least) per = r.least;
-    if (per > most) per = rows * seen / most <= 65536 ? most : rows * seen / 65536;
-    r.splits = (int)((seen + per - 1) / per);
+    r.waves = seen <= 32 ? 8 : 4;
+    r.least = r.waves;
+    if (seen <= 32) {
+        r.splits = 1;
+    } else {
+        const int64_t most = (s->batch > 1 ? 512 : 2048) / r.kt;
+        int64_t per = rows * seen / 1024;
+        if (per < r.least) per = r.least;
+        if (per > most) per = rows * seen / most <= 65536 ? most : rows * seen / 65536;
+        r.splits = (int)((seen + per - 1) / per);
+    }
     r.join = r.splits > 1 || accumulate;
     const int64_t parts = (int64_t)s->batch * heads * r.splits;
     r.o = r.join ? (size_t)parts * s->hd : 0;
@@ -654,8 +739,10 @@ extern "C" int ix_cache_attn(const struct ix_paged_cache* cache, const void* q, 
     const int64_t jblocks = oblocks + wblocks * cache->batch * cache->kv_heads;
     IX_CHECK_ARG((int64_t)cache->kv_heads * r.qtiles <= 65535 && jblocks < (1ll << 31), "ix_cache_attn: too many heads or tokens for one launch");
     const dim3 grid(r.splits, cache->kv_heads * r.qtiles, cache->batch);
-#define CACHE_GO(DT, D) cache_attn_kernel<DT, D><<<grid, kBlock, 0, stream>>>(p)
-#define CACHE_HD(DT) { if (hd == 32) CACHE_GO(DT, 32); else if (hd == 64) CACHE_GO(DT, 64); else CACHE_GO(DT, 128); }
+#define CACHE_GO(DT, D)                                                                       \
+    { if (r.waves == 8) cache_attn_kernel<DT, D, 8><<<grid, 512, 0, stream>>>(p);             \
+      else cache_attn_kernel<DT, D, 4><<<grid, 256, 0, stream>>>(p); }
+#define CACHE_HD(DT) { if (hd == 32) CACHE_GO(DT, 32) else if (hd == 64) CACHE_GO(DT, 64) else CACHE_GO(DT, 128) }
     if (cache->dtype == 0) CACHE_HD(0) else if (cache->dtype == 1) CACHE_HD(1) else CACHE_HD(2)
     IX_CHECK_LAUNCH("ix_cache_attn");
     if (r.join) {
@@ -689,11 +776,12 @@ extern "C" int ix_cache_compact(const struct ix_paged_cache* cache, const int* k
     p.left = left;
     p.budget = budget;
     p.row_bytes = cache->hd * (cache->dtype == 0 ? 4 : 2);
-    // whole rows while that gives a workgroup to every compute unit; else column slices down to 64 bytes
-    p.slice = p.row_bytes;
-    while (p.slice > 64 && (int64_t)cache->batch * cache->kv_heads * 2 * (p.row_bytes / p.slice) < 512) p.slice /= 2;
-    p.slices = p.row_bytes / p.slice;
-    compact_kernel<<<dim3(2 * p.slices + 1, cache->kv_heads, cache->batch), kBlock, 0, stream>>>(p);
+    // slices of 128 bytes (a cache line); of 64 where a row has no more, or where that leaves compute units without a workgroup
+    const bool narrow = p.row_bytes < 128 || (int64_t)cache->batch * cache->kv_heads * 2 * (p.row_bytes / 128) < 256;
+    p.slices = p.row_bytes / (narrow ? 64 : 128);
+    const dim3 grid(2 * p.slices + 1, cache->kv_heads, cache->batch);
+    if (narrow) compact_kernel<4><<<grid, kBlock, 0, stream>>>(p);
+    else compact_kernel<8><<<grid, kBlock, 0, stream>>>(p);
     IX_CHECK_LAUNCH("ix_cache_compact");
     return IX_OK;
 }

@@ -21,22 +21,29 @@ class _BandC(ctypes.Structure):   # struct ix_band of include/interactron_hip.h
                 [("scale", ctypes.c_float)])
 
 
+_NAMES = ("q", "k", "v", "q_lens", "kv_lens")
+
+
 def _dense_rows(t):
     """t, or a copy whose rows the kernels can read: last dimension dense, every row on 16 bytes"""
     per = 16 // t.element_size()
     sb, sl, sh, sd = t.stride()
-    if sd != 1 or sb % per or sl % per or sh % per or t.data_ptr() % 16:
+    if sd != 1 or sb % per or sl % per or sh % per or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _band(q, k, v, how):
-    window, sinks, causal, scale, q_lens, kv_lens = how
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _band(q, k, v, q_lens, kv_lens, window, sinks, causal, scale):
     B, Lq, H, D = q.shape
-    c = _BandC(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-               q_lens.data_ptr() if q_lens is not None else None, kv_lens.data_ptr() if kv_lens is not None else None,
-               _DTYPES[q.dtype], B, Lq, k.shape[1], H, k.shape[2], D, window, sinks, causal, scale)
-    return ctypes.byref(c)
+    qb, ql, qh, _ = q.stride()
+    kb, kl, kh, _ = k.stride()
+    vb, vl, vh, _ = v.stride()
+    return _BandC(q.data_ptr(), k.data_ptr(), v.data_ptr(), qb, ql, qh, kb, kl, kh, vb, vl, vh, _ptr(q_lens), _ptr(kv_lens),
+                  _DTYPES[q.dtype], B, Lq, k.shape[1], H, k.shape[2], D, window, sinks, causal, scale)
 
 
 class BandAttention(Function):
@@ -46,21 +53,25 @@ class BandAttention(Function):
 
     @staticmethod
     def forward(ctx, q, k, v, q_lens, kv_lens, window, sinks, causal, scale):
-        how = (window, sinks, causal, scale, q_lens, kv_lens)
-        s = _here((q, "q"), (k, "k"), (v, "v"), (q_lens, "q_lens"), (kv_lens, "kv_lens"))
+        s = _here(_NAMES, q, k, v, q_lens, kv_lens)
         recorded = not isinstance(ctx, _NullCtx) and any(ctx.needs_input_grad[:3])
-        B, Lq, H, D = q.shape
-        ctx.how, ctx.shapes = how[:4], (q.shape, k.shape, v.shape)
-        ctx.empty = 0 in q.shape or k.shape[1] == 0
+        shape = q.shape
+        ctx.empty = 0 in shape or k.shape[1] == 0
         if ctx.empty:   # nothing to see: zeros, and no gradient
             ctx.save_for_backward(q, k, v)
-            return q.new_zeros(q.shape)
+            return q.new_zeros(shape)
         q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
-        out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
-        lse = torch.empty((B, H, -(-Lq // 128) * 128), dtype=torch.float32, device=q.device) if recorded else None
-        _chk(_L().ix_band_attn_fwd(_band(q, k, v, how), out.data_ptr(), lse.data_ptr() if recorded else None, s), "ix_band_attn_fwd")
-        if recorded:
-            ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
+        band = _band(q, k, v, q_lens, kv_lens, window, sinks, causal, scale)
+        out, lse, rest = torch.empty(shape, dtype=q.dtype, device=q.device), None, None
+        if recorded:   # the rows' normalisers and, with 16-bit types, what rounding took from the output: for the gradients
+            lse = torch.empty(shape[0], shape[2], -(-shape[1] // 128) * 128, dtype=torch.float32, device=q.device)
+            if q.dtype is not torch.float32:
+                rest = torch.empty(shape, dtype=q.dtype, device=q.device)
+            ctx.how = (window, sinks, causal, scale)
+            ctx.save_for_backward(q, k, v, out, lse, rest, q_lens, kv_lens)
+        rc = _L().ix_band_attn_fwd(ctypes.byref(band), out.data_ptr(), _ptr(lse), _ptr(rest), s)
+        if rc:
+            _chk(rc, "ix_band_attn_fwd")
         return out
 
     @staticmethod
@@ -69,18 +80,23 @@ class BandAttention(Function):
             raise _lib.HipLibraryError("band_attention is differentiable once: no gradient of its gradient (create_graph=True)")
         need = ctx.needs_input_grad
         if ctx.empty:
-            return tuple(torch.zeros_like(t) if n else None for t, n in zip(ctx.saved_tensors, need)) + (None,) * 6
-        q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
-        do = _dense_rows(do.to(q.dtype))
-        s = _here((do, "the gradient"))
-        band = _band(q, k, v, ctx.how + (q_lens, kv_lens))
+            return tuple([torch.zeros_like(t) if n else None for t, n in zip(ctx.saved_tensors, need)]) + (None,) * 6
+        q, k, v, out, lse, rest, q_lens, kv_lens = ctx.saved_tensors
+        if do.dtype is not q.dtype:
+            do = do.to(q.dtype)
+        do = _dense_rows(do)
+        s = _here(("the gradient",), do)
+        band = ctypes.byref(_band(q, k, v, q_lens, kv_lens, *ctx.how))
         n = ctypes.c_size_t(0)
         _chk(_L().ix_workspace_bytes_band_attn_bwd(band, ctypes.byref(n)), "ix_workspace_bytes_band_attn_bwd")
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _chk(_L().ix_band_attn_bwd(band, out.data_ptr(), lse.data_ptr(), do.data_ptr(), *do.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                   ws.data_ptr(), n.value, s), "ix_band_attn_bwd")
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None) + (None,) * 6
+        dq, dk, dv = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+        gb, gl, gh, _ = do.stride()
+        rc = _L().ix_band_attn_bwd(band, out.data_ptr(), _ptr(rest), lse.data_ptr(), do.data_ptr(), gb, gl, gh, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                   ws.data_ptr(), n.value, s)
+        if rc:
+            _chk(rc, "ix_band_attn_bwd")
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None, None, None
 
 
 def band_attention(q, k, v, window=None, sinks=0, causal=True, scale=None, q_lens=None, kv_lens=None):

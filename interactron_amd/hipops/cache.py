@@ -11,6 +11,7 @@ alone (the lengths stay on the device) and may be captured into a HIP graph.  (T
 over all frames again for every new one, models/interactron.py:166-190.)
 """
 import ctypes
+import math
 
 import torch
 
@@ -20,6 +21,8 @@ from .core import _L, _chk, _stream
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _HEAD_DIMS = (32, 64, 128)
+_PAGES = (16, 32, 64, 128, 256, 512, 1024)
+_CACHE_NAMES = ("cache keys", "cache values", "the page table", "the lengths", "the weights")
 
 
 class _CacheC(ctypes.Structure):   # struct ix_paged_cache of include/interactron_hip.h
@@ -28,23 +31,31 @@ class _CacheC(ctypes.Structure):   # struct ix_paged_cache of include/interactro
                 ("page", ctypes.c_int), ("hd", ctypes.c_int), ("batch", ctypes.c_int), ("pages", ctypes.c_int)]
 
 
-def _here(*named):
-    """The current stream, after checking that every (tensor, name) lives on the device this process computes on."""
-    for t, name in named:
-        if t is not None and not t.is_cuda:
-            raise _lib.HipLibraryError("%s must live on the GPU: the HIP path has no CPU fallback" % name)
-    s = _stream()
-    dev = core._dev[0] if core._dev[0] is not None else torch.cuda.current_device()
-    for t, name in named:
-        if t is not None and t.device.index != dev:
-            raise _lib.HipLibraryError("%s lives on cuda:%d but this process computes on cuda:%d (one process per GPU)" % (name, t.device.index, dev))
-    if torch.cuda.current_device() != dev:
-        raise _lib.HipLibraryError("the current device is cuda:%d but this process computes on cuda:%d (one process per GPU)" % (torch.cuda.current_device(), dev))
-    return s
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _here(names, *ts):
+    """The current stream, after checking that every tensor lives on the device this process computes on."""
+    dev = core._dev[0]
+    if dev is None:
+        for t, name in zip(ts, names):
+            if t is not None and not t.is_cuda:
+                raise _lib.HipLibraryError("%s must live on the GPU: the HIP path has no CPU fallback" % name)
+        _stream()   # (binds the device)
+        dev = torch.cuda.current_device() if core._dev[0] is None else core._dev[0]
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            name = next(n for x, n in zip(ts, names) if x is t)
+            if not t.is_cuda:
+                raise _lib.HipLibraryError("%s must live on the GPU: the HIP path has no CPU fallback" % name)
+            raise _lib.HipLibraryError("%s lives on cuda:%d but this process computes on cuda:%d (one process per GPU)" % (name, t.get_device(), dev))
+    if _device() != dev:
+        raise _lib.HipLibraryError("the current device is cuda:%d but this process computes on cuda:%d (one process per GPU)" % (_device(), dev))
+    return _stream()
 
 
 def _whole(t, name, dtype, shape):
-    if t.dtype != dtype or tuple(t.shape) != shape:
+    if t.dtype != dtype or t.shape != shape:
         raise ValueError("%s must be %s %s, got %s %s" % (name, dtype, list(shape), t.dtype, list(t.shape)))
     if not t.is_contiguous():
         raise ValueError("%s must be contiguous: it is used in place" % name)
@@ -66,52 +77,53 @@ class PagedCache:
     lens     int32 [batch]: tokens held
     weight   float32 [batch, kv_heads, pages * page] or None: the attention each token has had so far
     """
-    __slots__ = ("k", "v", "table", "lens", "weight", "kv_heads", "hd", "page", "batch", "pages", "capacity", "c", "ref", "_ws")
+    __slots__ = ("k", "v", "table", "lens", "weight", "kv_heads", "hd", "page", "batch", "pages", "capacity", "c", "ref")
 
     def __init__(self, k, v, table, lens, weight=None):
-        if k.dim() != 4 or k.dtype not in _DTYPES:
-            raise ValueError("cache keys must be [pages_total, kv_heads, page, hd] in float32, bfloat16 or float16, got %s %s" % (k.dtype, list(k.shape)))
-        total, kv, page, hd = k.shape
+        shape, code = k.shape, _DTYPES.get(k.dtype)
+        if len(shape) != 4 or code is None:
+            raise ValueError("cache keys must be [pages_total, kv_heads, page, hd] in float32, bfloat16 or float16, got %s %s" % (k.dtype, list(shape)))
+        total, kv, page, hd = shape
         if hd not in _HEAD_DIMS:
             raise ValueError("a cache of head dim %d: %s are supported" % (hd, _HEAD_DIMS))
-        if page < 16 or page > 1024 or page & (page - 1):
+        if page not in _PAGES:
             raise ValueError("a page of %d tokens: powers of two from 16 to 1024 are supported" % page)
-        if table.dim() != 2 or 0 in table.shape or 0 in k.shape:
-            raise ValueError("an empty cache, or a page table that is not [batch, pages]: %s, %s" % (list(k.shape), list(table.shape)))
+        if table.dim() != 2 or not table.numel() or not k.numel():
+            raise ValueError("an empty cache, or a page table that is not [batch, pages]: %s, %s" % (list(shape), list(table.shape)))
         B, pages = table.shape
-        _whole(k, "cache keys", k.dtype, (total, kv, page, hd))
-        _whole(v, "cache values", k.dtype, (total, kv, page, hd))
+        _whole(k, "cache keys", k.dtype, shape)
+        _whole(v, "cache values", k.dtype, shape)
         _whole(table, "the page table", torch.int32, (B, pages))
         _whole(lens, "the lengths", torch.int32, (B,))
         if weight is not None:
             _whole(weight, "the weights", torch.float32, (B, kv, pages * page))
         if B > 65535 or kv > 1024 or pages * page >= 1 << 30 or total >= 1 << 31:
             raise ValueError("a cache of %d sequences, %d key heads, %d tokens a sequence is too large" % (B, kv, pages * page))
-        _here((k, "cache keys"), (v, "cache values"), (table, "the page table"), (lens, "the lengths"), (weight, "the weights"))
-        if k.data_ptr() % 16 or v.data_ptr() % 16:
+        _here(_CACHE_NAMES, k, v, table, lens, weight)
+        pk, pv = k.data_ptr(), v.data_ptr()
+        if (pk | pv) & 15:
             raise ValueError("cache keys and values must start on 16 bytes")
         self.k, self.v, self.table, self.lens, self.weight = k, v, table, lens, weight
         self.kv_heads, self.hd, self.page, self.batch, self.pages, self.capacity = kv, hd, page, B, pages, pages * page
-        self.c = _CacheC(k.data_ptr(), v.data_ptr(), table.data_ptr(), lens.data_ptr(), weight.data_ptr() if weight is not None else None, total,
-                         _DTYPES[k.dtype], kv, page, hd, B, pages)
+        self.c = _CacheC(pk, pv, table.data_ptr(), lens.data_ptr(), None if weight is None else weight.data_ptr(), total, code, kv, page, hd, B, pages)
         self.ref = ctypes.byref(self.c)
-        self._ws = {}   # workspace bytes by call signature
 
 
-def _rows(t, name, cache, shape, dims):
-    """t with rows that the kernels can read: last dimension dense, every row on 16 bytes (copied where it is not)"""
-    if t.dtype != cache.k.dtype or tuple(t.shape) != shape:
+def _rows(t, name, cache, shape):
+    """t with rows that the kernels can read, and its strides: last dimension dense, every row on 16 bytes (copied where it is not)"""
+    if t.dtype != cache.k.dtype or t.shape != shape:
         raise ValueError("%s must be %s %s like the cache, got %s %s" % (name, cache.k.dtype, list(shape), t.dtype, list(t.shape)))
-    per = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(t.stride(d) % per for d in range(dims)):
-        t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    strides, per = t.stride(), 16 // t.element_size()
+    if strides[-1] != 1 or t.data_ptr() & 15 or any([x % per for x in strides[:-1]]):
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = t.stride()
+    return t, strides
 
 
 def _per_sequence(t, name, cache):
     if t is not None:
         _whole(t, name, torch.int32, (cache.batch,))
-    return t
+        return t.data_ptr()
 
 
 def cache_append(cache, k, v, counts=None, at=None):
@@ -124,12 +136,29 @@ def cache_append(cache, k, v, counts=None, at=None):
         raise ValueError("new keys must be [batch, tokens, kv_heads, hd], got %s" % list(k.shape))
     T = k.shape[1]
     shape = (cache.batch, T, cache.kv_heads, cache.hd)
-    k, v = _rows(k, "new keys", cache, shape, 3), _rows(v, "new values", cache, shape, 3)
-    _per_sequence(counts, "counts", cache)
-    _per_sequence(at, "at", cache)
-    s = _here((k, "new keys"), (v, "new values"), (counts, "counts"), (at, "at"))
-    _chk(_L().ix_cache_append(cache.ref, k.data_ptr(), v.data_ptr(), T, *k.stride()[:3], *v.stride()[:3],
-                              counts.data_ptr() if counts is not None else None, at.data_ptr() if at is not None else None, s), "ix_cache_append")
+    k, (kb, kt, kh, _) = _rows(k, "new keys", cache, shape)
+    v, (vb, vt, vh, _) = _rows(v, "new values", cache, shape)
+    n, start = _per_sequence(counts, "counts", cache), _per_sequence(at, "at", cache)
+    s = _here(("new keys", "new values", "counts", "at"), k, v, counts, at)
+    rc = _L().ix_cache_append(cache.ref, k.data_ptr(), v.data_ptr(), T, kb, kt, kh, vb, vt, vh, n, start, s)
+    if rc:
+        _chk(rc, "ix_cache_append")
+
+
+_ws_bytes = {}   # workspace of ix_cache_attn by sizes
+
+
+def _attention_ws(cache, H, window, sinks, accumulate):
+    c = cache.c
+    key = (c.dtype, c.kv_heads, c.page, c.hd, c.batch, c.pages, H, window, sinks, accumulate)
+    need = _ws_bytes.get(key)
+    if need is None:
+        n = ctypes.c_size_t(0)
+        _chk(_L().ix_workspace_bytes_cache_attn(cache.ref, H, window, sinks, accumulate, ctypes.byref(n)), "ix_workspace_bytes_cache_attn")
+        if len(_ws_bytes) >= 4096:
+            _ws_bytes.clear()
+        need = _ws_bytes[key] = n.value
+    return need
 
 
 def cache_attention(q, cache, scale=None, window=None, sinks=0, accumulate=False):
@@ -143,23 +172,23 @@ def cache_attention(q, cache, scale=None, window=None, sinks=0, accumulate=False
     H = q.shape[1]
     if H > 4096:
         raise ValueError("%d query heads: at most 4096 are supported" % H)
-    q = _rows(q, "q", cache, (cache.batch, H, cache.hd), 2)
-    w, sinks = 0 if window is None else _count(window, "window", 1), _count(sinks, "sinks")
-    if accumulate and cache.weight is None:
-        raise ValueError("accumulate: the cache holds no weights")
+    shape = (cache.batch, H, cache.hd)
     if q.requires_grad and torch.is_grad_enabled():
         raise _lib.HipLibraryError("cache_attention has no backward: call it under torch.no_grad()")
-    s = _here((q, "q"))
-    key = (H, w, sinks, bool(accumulate))
-    need = cache._ws.get(key)
-    if need is None:
-        n = ctypes.c_size_t(0)
-        _chk(_L().ix_workspace_bytes_cache_attn(cache.ref, H, w, sinks, int(bool(accumulate)), ctypes.byref(n)), "ix_workspace_bytes_cache_attn")
-        need = cache._ws[key] = n.value
-    out = torch.empty((cache.batch, H, cache.hd), dtype=q.dtype, device=q.device)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None   # (a buffer per call: calls on other streams and captured graphs share none)
-    _chk(_L().ix_cache_attn(cache.ref, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), H, cache.hd ** -0.5 if scale is None else float(scale),
-                            w, sinks, int(bool(accumulate)), ws.data_ptr() if ws is not None else None, need, s), "ix_cache_attn")
+    q, (qb, qh, _) = _rows(q, "q", cache, shape)
+    w, sinks, accumulate = 0 if window is None else _count(window, "window", 1), _count(sinks, "sinks"), 1 if accumulate else 0
+    if accumulate and cache.weight is None:
+        raise ValueError("accumulate: the cache holds no weights")
+    scale = cache.hd ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be a finite number, got %r" % scale)
+    s = _here(("q",), q)
+    out, ws, need = torch.empty(shape, dtype=q.dtype, device=q.device), None, _attention_ws(cache, H, w, sinks, accumulate)
+    if need:   # (a buffer per call: calls on other streams and captured graphs share none)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    rc = _L().ix_cache_attn(cache.ref, q.data_ptr(), qb, qh, out.data_ptr(), H, scale, w, sinks, accumulate, None if ws is None else ws.data_ptr(), need, s)
+    if rc:
+        _chk(rc, "ix_cache_attn")
     return out
 
 
@@ -178,7 +207,7 @@ def cache_select(weight, lens, budget, sinks=0, recent=0):
     budget, sinks, recent = _count(budget, "budget", 1), _count(sinks, "sinks"), _count(recent, "recent")
     if budget > cap or sinks + recent > budget:
         raise ValueError("a budget of %d tokens for a capacity of %d, of which %d first and %d last ones" % (budget, cap, sinks, recent))
-    s = _here((weight, "weight"), (lens, "lens"))
+    s = _here(("weight", "lens"), weight, lens)
     kept = torch.empty((B, kv, budget), dtype=torch.int32, device=weight.device)
     left = torch.empty(B, dtype=torch.int32, device=weight.device)
     _chk(_L().ix_cache_select(weight.data_ptr(), lens.data_ptr(), kept.data_ptr(), left.data_ptr(), B, kv, cap, budget, sinks, recent, s), "ix_cache_select")
@@ -197,7 +226,7 @@ def cache_compact(cache, kept, left):
         raise ValueError("kept names %d tokens, the capacity is %d" % (kept.shape[2], cache.capacity))
     if left.data_ptr() == cache.lens.data_ptr():
         raise ValueError("left must not be the cache's own lengths")
-    s = _here((kept, "kept"), (left, "left"))
+    s = _here(("kept", "left"), kept, left)
     _chk(_L().ix_cache_compact(cache.ref, kept.data_ptr(), left.data_ptr(), kept.shape[2], s), "ix_cache_compact")
 
 
