@@ -539,7 +539,8 @@ int ix_adam_step_f32(float* p, float* g, float* m, float* v, int64_t n, float lr
  * q_lens, kv_lens int32 [batch] (null: Lq, Lk): rows behind them are never read and come back as zeros.  A query that sees nothing
  * gives zeros and has no gradient.  Keys and values that a query does not see have to be finite where they lie inside the lengths.
  *   ix_band_attn_fwd : out [batch][Lq][heads][hd] dense; for the gradients (may be null) lse f32 [batch][heads][pitch], base 2 (pitch
- *                      from ix_band_attn_lse_pitch), and rest like out: what its rounding to 16 bits took away (not with f32)
+ *                      from ix_band_attn_lse_pitch), and rest like out: what its rounding to 16 bits took away (not with f32).  Few
+ *                      rows over many keys go in pieces that are joined: workspace of ix_workspace_bytes_band_attn_fwd bytes (often 0)
  *   ix_band_attn_bwd : dq, dk, dv (dense, like q, k, v) from out, rest, lse and d_out [batch][Lq][heads][hd] by strides g_*; sums in f32,
  *                      in a fixed order (no atomics); workspace of ix_workspace_bytes_band_attn_bwd bytes, 16-byte aligned */
 struct ix_band {
@@ -549,7 +550,9 @@ struct ix_band {
     int dtype, batch, Lq, Lk, heads, kv_heads, hd, window, sinks, causal;
     float scale;
 };
-int ix_band_attn_fwd(const struct ix_band* band_host, void* out, float* lse, void* rest, ix_stream_t stream);
+int ix_workspace_bytes_band_attn_fwd(const struct ix_band* band_host, size_t* out_host);
+int ix_band_attn_fwd(const struct ix_band* band_host, void* out, float* lse, void* rest, void* workspace, size_t workspace_bytes,
+                     ix_stream_t stream);
 int ix_band_attn_lse_pitch(int Lq, int64_t* out_host);
 int ix_workspace_bytes_band_attn_bwd(const struct ix_band* band_host, size_t* out_host);
 int ix_band_attn_bwd(const struct ix_band* band_host, const void* out, const void* rest, const float* lse, const void* d_out, int64_t g_sb,

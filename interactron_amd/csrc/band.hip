@@ -21,8 +21,7 @@ constexpr int kBlock = 256, kWaves = 4;
 constexpr int kFar = 1 << 30;   // an unlimited band (lengths stay below 2^28)
 
 // owner rows of a wave: two blocks of 16 with 16-bit operands, one with f32 (twice the registers an element)
-constexpr int owner_blocks(int dt) { return dt == 0 ? 1 : 2; }
-constexpr int owner_rows(int dt) { return 16 * owner_blocks(dt) * kWaves; }
+constexpr int owner_rows(int nb) { return 16 * nb * kWaves; }
 constexpr int key_tile(int dt) { return dt == 0 ? 32 : 64; }
 constexpr int query_tile(int dt, int hd) { return dt == 0 || hd == 128 ? 32 : 64; }
 
@@ -30,7 +29,7 @@ constexpr int query_tile(int dt, int hd) { return dt == 0 || hd == 128 ? 32 : 64
 // 32-byte pairs of a row change places by the row's number, so that eight neighbouring rows' pieces lie in different banks for both ways
 // of reading.  f32: also the four rows 4 apart that a transposed read takes at once.
 template <int DT, int D> struct Img {
-    static constexpr int EB = SeqT<DT>::bytes, ROW = D * EB, PAIRS = ROW / 32, SWEEP = ROW >= 256 ? 1 : 256 / ROW, KS = D / 32, DB = D / 16;
+    static constexpr int EB = SeqT<DT>::bytes, ROW = D * EB, PAIRS = ROW / 32, SWEEP = ROW >= 256 ? 1 : 256 / ROW, KS = D / 32, DB = D / 16, DN = DB < 4 ? DB : 4;
     __device__ static __forceinline__ int turn(int row) {
         if constexpr (DT == 0) return (((row >> 2) & 3) << 1 | (row & 1)) & (PAIRS - 1);
         else return (row / SWEEP) & (PAIRS - 1);
@@ -50,64 +49,91 @@ template <int DT, int D> struct Img {
         }
         return f;
     }
-    // column d = 16 db + n of rows row0 + 4 g + i and row0 + 16 + 4 g + i (row0 a multiple of 32)
-    __device__ static __forceinline__ Frag<DT> col_frag(const unsigned char* img, int row0, int db, int n, int g) {
-        Frag<DT> f;
+    // columns d = 16 db + n of rows row0 + 4 g + i and row0 + 16 + 4 g + i (row0 a multiple of 32), for DN values of db from db0 on.
+    // The transposing reads stand in one block with their wait: the compiler would let each of them wait for every request into LDS that
+    // is still on its way, those of the next tiles too.
+    template <int DN> __device__ static __forceinline__ void col_frags(Frag<DT> (&f)[DN], const unsigned char* img, int row0, int db0, int n, int g) {
         if constexpr (DT == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = row0 + 16 * (i / 4) + 4 * g + i % 4;
-                f.w[i] = *reinterpret_cast<const unsigned*>(img + row * ROW + (((2 * db + (n >> 3)) ^ turn(row)) << 5) + ((n & 7) << 2));
-            }
+            for (int db = 0; db < DN; ++db)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = row0 + 16 * (i / 4) + 4 * g + i % 4;
+                    f[db].w[i] = *reinterpret_cast<const unsigned*>(img + row * ROW + (((2 * (db0 + db) + (n >> 3)) ^ turn(row)) << 5) + ((n & 7) << 2));
+                }
         } else {
-            const int row = row0 + 4 * g + (n >> 2);
-            const unsigned char* p = img + row * ROW + ((db ^ turn(row)) << 5) + ((n & 3) << 3);
-            typedef s16x4 __attribute__((address_space(3))) lds4;
-            const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p)));
-            const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * ROW)));
-            f.w[0] = a.x; f.w[1] = a.y; f.w[2] = b.x; f.w[3] = b.y;
+            const int row = row0 + 4 * g + (n >> 2), t = turn(row);
+            const unsigned at = (unsigned)(uintptr_t)(const unsigned char __attribute__((address_space(3)))*)img + row * ROW + ((n & 3) << 3);
+            u32x2 x[DN][2];
+            static_assert(DN == 2 || DN == 4, "");
+#ifdef __HIP_DEVICE_COMPILE__   // (the host's pass does not know the registers' constraint)
+            if constexpr (DN == 2) {
+                asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+                             "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+                             : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1])
+                             : "v"(at + ((db0 ^ t) << 5)), "v"(at + (((db0 + 1) ^ t) << 5)), "n"(16 * ROW) : "memory");
+            } else {
+                asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+                             "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+                             "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+                             "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                             : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[2][0]), "=&v"(x[2][1]), "=&v"(x[3][0]), "=&v"(x[3][1])
+                             : "v"(at + ((db0 ^ t) << 5)), "v"(at + (((db0 + 1) ^ t) << 5)), "v"(at + (((db0 + 2) ^ t) << 5)), "v"(at + (((db0 + 3) ^ t) << 5)),
+                               "n"(16 * ROW) : "memory");
+            }
+#endif
+#pragma unroll
+            for (int db = 0; db < DN; ++db) { f[db].w[0] = x[db][0].x; f[db].w[1] = x[db][0].y; f[db].w[2] = x[db][1].x; f[db].w[3] = x[db][1].y; }
         }
-        return f;
     }
 };
 static_assert(Img<1, 128>::PAIRS == 8 && Img<1, 32>::SWEEP == 4, "image geometry");
 
-// a tile of ROWS rows on its way from memory to LDS: requested before the arithmetic of the tile in front of it, stored after it
-template <int DT, int D, int ROWS> struct Stage {
-    static constexpr int CH = Img<DT, D>::ROW / 16, N = ROWS * CH / kBlock;
+// A tile of ROWS rows from memory to LDS without registers: every lane names the 16 bytes that belong at its place of the image
+// (the image's order is the lanes'), rows from `rows` on read as zeros (they lie behind the descriptor's end).
+typedef void __attribute__((address_space(3))) lds_void;
+template <int DT, int D, int ROWS> struct Dma {
+    static constexpr int CH = Img<DT, D>::ROW / 16, N = ROWS * CH / kBlock;   // requests of a wave
     static_assert(ROWS * CH % kBlock == 0, "a tile is whole passes of the workgroup");
-    u32x4 r[N];
-    __device__ __forceinline__ void load(const unsigned char* base, int64_t stride, int row0, int rows) {
+    int at[N];
+    const unsigned char* base;
+    int64_t stride;
+    __device__ __forceinline__ Dma(const unsigned char* base_, int64_t stride_, int wave, int lane) : base(base_), stride(stride_) {
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-            const int c = threadIdx.x + u * kBlock, row = row0 + c / CH;
-            r[u] = row < rows ? *reinterpret_cast<const u32x4*>(base + row * stride + (c % CH) * 16) : u32x4{0, 0, 0, 0};
+            const int place = (wave * N + u) * 64 + lane, row = place / CH, c = place % CH;
+            at[u] = row * (int)stride + ((((c >> 1) ^ Img<DT, D>::turn(row)) << 1 | (c & 1)) << 4);
         }
     }
-    __device__ __forceinline__ void store(unsigned char* img) const {
+    __device__ __forceinline__ void issue(unsigned char* img, int wave, int row0, int rows) const {
+        const int64_t end = row0 < rows ? (int64_t)(rows - row0 - 1) * stride + Img<DT, D>::ROW : 0;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + row0 * stride), 0, (int)min(end, (int64_t)0x7ffffff0), 0x00020000);
 #pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int c = threadIdx.x + u * kBlock;
-            *reinterpret_cast<u32x4*>(img + Img<DT, D>::chunk(c / CH, c % CH)) = r[u];
-        }
+        for (int u = 0; u < N; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(img + (wave * N + u) * 1024), 16, at[u], 0, 0, 0);
     }
 };
+// this wave's requests but the newest N have landed, and it has read what it wanted of the other stages; then everybody's and everybody
+template <int N> __device__ __forceinline__ void landed() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// stages of the ring: three (requests two tiles ahead) where a workgroup's LDS stays within 48 KB, else two
+constexpr int stages(int bytes) { return 3 * bytes <= 49152 ? 3 : 2; }
 
 struct BandArgs {
     const unsigned char *q, *k, *v, *go, *o, *o_rest;
     int64_t qb, ql, qh, kb, kl, kh, vb, vl, vh, gb, gl, gh;   // bytes
     unsigned char *out, *rest, *dq, *dk, *dv;                 // dense; rest: what rounding the output to 16 bits took away, in 16 bits
-    float *lse, *delta, *part;                                // [B][H][Lp] base-2 normalisers (+inf: nothing visible) and delta; partial sums
+    float *lse, *delta, *part, *part_ml;                      // [B][H][Lp] base-2 normalisers (+inf: nothing visible) and delta; partial sums
     const int *q_lens, *kv_lens;
     int B, Lq, Lk, Lp, H, kv, left, right, sinks, causal;
     int wide_blocks, wide_splits, splits, key_groups;         // dk / dv: see the host side; workgroups of theirs
+    int fwd_splits;                                           // forward: pieces of a block's key tiles
     float c2, scale;                                          // |scale| log2(e), scale
     unsigned flip;                                            // sign bits of a fragment's register where scale < 0
     __device__ __forceinline__ int m(int b) const { return q_lens ? min(max(q_lens[b], 0), Lq) : Lq; }
     __device__ __forceinline__ int n(int b) const { return kv_lens ? min(max(kv_lens[b], 0), Lk) : Lk; }
-    __device__ __forceinline__ bool sees(int p_, int j, int n_) const {
-        return (j < n_) & (((j >= p_ - left) & (j <= p_ + right)) | ((j < sinks) & (!causal | (j <= p_))));
-    }
     // every pair of p0 .. p1 and j0 .. j1 sees each other (apart from j < n)
     __device__ __forceinline__ bool all_see(int p0, int p1, int j0, int j1) const {
         return (j0 >= p1 - left && j1 <= p0 + right) || (j1 < sinks && (!causal || j1 <= p0));
@@ -116,6 +142,25 @@ struct BandArgs {
         return (j1 < p0 - left || j0 > p1 + right) && (j0 >= sinks || (causal && j0 > p1));
     }
 };
+
+// The streamed rows x that go with one owner row: lo <= x <= lo + width, or x < first.
+struct Range {
+    int lo, first;
+    unsigned width;
+    __device__ __forceinline__ bool in(int x) const { return (unsigned)(x - lo) <= width; }
+};
+// the keys that a query at p sees among n
+__device__ __forceinline__ Range keys_of(const BandArgs& a, int p, int n) {
+    const int hi = min(n - 1, p + a.right), lo = p - a.left;
+    const bool some = lo <= hi;
+    return Range{some ? lo : kFar, max(0, min(n, a.causal ? min(a.sinks, p + 1) : a.sinks)), some ? (unsigned)(hi - lo) : 0u};
+}
+// the positions of the queries that see key j
+__device__ __forceinline__ Range queries_of(const BandArgs& a, int j) {
+    const bool to_all = j < a.sinks;
+    const int lo = to_all ? (a.causal ? j : -kFar) : j - a.right;
+    return Range{lo, 0, to_all ? 2u * kFar : (unsigned)a.left + (unsigned)a.right};
+}
 
 // (batch, head) of workgroup x of `total`: neighbouring heads -- which share keys -- on one XCD (workgroups go round the eight of them)
 __device__ __forceinline__ int spread_heads(int x, int total) { return total % 8 == 0 ? (x % 8) * (total / 8) + x / 8 : x; }
@@ -172,6 +217,23 @@ template <int DT> __device__ __forceinline__ void store4(unsigned char* p, const
     else *reinterpret_cast<u32x2*>(p) = u32x2{seq_pack<DT>(x[0], x[1]), seq_pack<DT>(x[2], x[3])};
 }
 
+// four values of the output, and of what rounding takes from them
+template <int DT> __device__ __forceinline__ void store_out(const BandArgs& a, int64_t at, const f32x4& x) {
+    store4<DT>(a.out + at, x);
+    if constexpr (DT != 0) {
+        if (a.rest) {
+            f32x4 y;
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+                const unsigned w = seq_pack<DT>(x[r], x[r + 1]);
+                y[r] = x[r] - seq_lo<DT>(w);
+                y[r + 1] = x[r + 1] - seq_hi<DT>(w);
+            }
+            store4<DT>(a.rest + at, y);
+        }
+    }
+}
+
 // fp16: gradients of scores may lie anywhere in the f32 range.  They are rounded as dz F, F a power of two of the accumulator's column
 // that only falls: where a value would reach 2^15 it is lowered until the value lies in [2^14, 2^15) and the sum so far is rescaled.
 template <int DB> __device__ __forceinline__ void fit16(float top, float& F, f32x4 (&acc)[DB]) {
@@ -198,10 +260,10 @@ constexpr float kFirstF = 1099511627776.f;   // 2^40
 constexpr float kSlack = 8.f;
 
 template <int DT, int D, int NB, int TB>
-__global__ __launch_bounds__(kBlock, 2) void band_fwd_kernel(BandArgs a) {
+__device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) {
     typedef Img<DT, D> I;
-    constexpr int ROWS = 16 * NB * kWaves, SB = TB / 16, BYTES = TB * I::ROW;
-    __shared__ __attribute__((aligned(256))) unsigned char lds[2][2][BYTES];
+    constexpr int ROWS = 16 * NB * kWaves, SB = TB / 16, BYTES = TB * I::ROW, STG = stages(2 * BYTES);
+    auto lds = reinterpret_cast<unsigned char (*)[2][BYTES]>(mem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
     const int bh = spread_heads(blockIdx.x, a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.kv);
     const int blk = a.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y, i0 = blk * ROWS;   // (causal: the longest rows first)
@@ -222,22 +284,22 @@ __global__ __launch_bounds__(kBlock, 2) void band_fwd_kernel(BandArgs a) {
         owner_frags<DT, D, NB>(qf, a.q + b * a.qb + h * a.qh, a.ql, iw, m, n16, g, a.flip);
         const unsigned char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
         const int pw0 = iw + shift, pw1 = min(iw + 16 * NB, m) - 1 + shift;
-        Stage<DT, D, TB> sk, sv;
-        if (kt.count) {
-            sk.load(kp, a.kl, kt.tile(0) * TB, n);
-            sv.load(vp, a.vl, kt.tile(0) * TB, n);
-            sk.store(lds[0][0]);
-            sv.store(lds[0][1]);
-        }
-        __syncthreads();
-        for (int t = 0; t < kt.count; ++t) {
-            const unsigned char *ki = lds[t & 1][0], *vi = lds[t & 1][1];
+        const Dma<DT, D, TB> dk(kp, a.kl, wave, lane), dv(vp, a.vl, wave, lane);
+        auto issue = [&](int t) {
+            const int row0 = kt.tile(t) * TB, st = t % STG;
+            dk.issue(lds[st][0], wave, row0, n);
+            dv.issue(lds[st][1], wave, row0, n);
+        };
+        const int t0 = kt.count * blockIdx.z / a.fwd_splits, t1 = kt.count * (blockIdx.z + 1) / a.fwd_splits;
+#pragma unroll
+        for (int t = 0; t < STG - 1; ++t)
+            if (t0 + t < t1) issue(t0 + t);
+        for (int t = t0; t < t1; ++t) {
+            const unsigned char *ki = lds[t % STG][0], *vi = lds[t % STG][1];
             const int j0 = kt.tile(t) * TB;
-            const bool more = t + 1 < kt.count;
-            if (more) {
-                sk.load(kp, a.kl, kt.tile(t + 1) * TB, n);
-                sv.load(vp, a.vl, kt.tile(t + 1) * TB, n);
-            }
+            if (STG == 3 && t + 1 < t1) landed<2 * Dma<DT, D, TB>::N>();
+            else landed<0>();
+            if (t + STG - 1 < t1) issue(t + STG - 1);
             if (iw < m && !a.none_sees(pw0, pw1, j0, j0 + TB - 1)) {
                 f32x4 s[NB][SB];
 #pragma unroll
@@ -252,15 +314,25 @@ __global__ __launch_bounds__(kBlock, 2) void band_fwd_kernel(BandArgs a) {
                     }
                 }
                 if (j0 + TB > n || !a.all_see(pw0, pw1, j0, j0 + TB - 1)) {
+                    const bool firsts = j0 < a.sinks;   // (uniform: most masked tiles have no first keys)
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const Range r = keys_of(a, iw + 16 * nb + n16 + shift, n);
+                        if (firsts) {
 #pragma unroll
-                        for (int sb = 0; sb < SB; ++sb)
+                            for (int sb = 0; sb < SB; ++sb)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const bool see = a.sees(iw + 16 * nb + n16 + shift, j0 + 16 * sb + 4 * g + r, n);
-                                s[nb][sb][r] = see ? s[nb][sb][r] : -INFINITY;
-                            }
+                                for (int e = 0; e < 4; ++e) {
+                                    const int j = j0 + 4 * g + 16 * sb + e;
+                                    s[nb][sb][e] = r.in(j) | (j < r.first) ? s[nb][sb][e] : -INFINITY;
+                                }
+                        } else {
+#pragma unroll
+                            for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) s[nb][sb][e] = r.in(j0 + 4 * g + 16 * sb + e) ? s[nb][sb][e] : -INFINITY;
+                        }
+                    }
                 }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
@@ -269,8 +341,9 @@ __global__ __launch_bounds__(kBlock, 2) void band_fwd_kernel(BandArgs a) {
                     for (int sb = 0; sb < SB; ++sb)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[nb][sb][r]);
-                    mx = seq_max_g(mx) * a.c2;
-                    if (__builtin_amdgcn_ballot_w64(mx > top[nb] + kSlack)) {
+                    mx *= a.c2;
+                    if (__builtin_amdgcn_ballot_w64(mx > top[nb] + kSlack)) {   // (each lane by its own keys: no exchange where nobody exceeds)
+                        mx = seq_max_g(mx);
                         const float up = fmaxf(top[nb], mx), down = up == -INFINITY ? 1.f : seq_exp2(top[nb] - up);
                         top[nb] = up;
                         sum[nb] *= down;
@@ -292,53 +365,77 @@ __global__ __launch_bounds__(kBlock, 2) void band_fwd_kernel(BandArgs a) {
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) pf[nb] = as_frag<DT>(s[nb][2 * kk], s[nb][2 * kk + 1]);
 #pragma unroll
-                    for (int db = 0; db < I::DB; ++db) {
-                        const Frag<DT> vf = I::col_frag(vi, 32 * kk, db, n16, g);
+                    for (int d0 = 0; d0 < I::DB; d0 += I::DN) {
+                        Frag<DT> vf[I::DN];
+                        I::col_frags(vf, vi, 32 * kk, d0, n16, g);
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) o[nb][db] = seq_mma<DT>(vf, pf[nb], o[nb][db]);
+                        for (int db = 0; db < I::DN; ++db)
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) o[nb][d0 + db] = seq_mma<DT>(vf[db], pf[nb], o[nb][d0 + db]);
                     }
                 }
             }
-            if (more) {
-                sk.store(lds[(t + 1) & 1][0]);
-                sv.store(lds[(t + 1) & 1][1]);
-            }
-            __syncthreads();
         }
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const int i = iw + 16 * nb + n16;
         const float total = seq_sum_g(sum[nb]);
+        if (a.fwd_splits > 1) {   // what this piece has, for band_join_kernel
+            if (i >= a.Lq) continue;
+            const int64_t at = ((int64_t)bh * a.Lq + i) * a.fwd_splits + blockIdx.z;
+            if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{top[nb], total};
+#pragma unroll
+            for (int db = 0; db < I::DB; ++db) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * db + 4 * g) = o[nb][db];
+            continue;
+        }
         const bool none = i >= m || total == 0.f;
         const float inv = 1.f / total;
         if (a.lse && g == 0 && i < a.Lp) a.lse[(int64_t)bh * a.Lp + i] = none ? INFINITY : top[nb] + __log2f(total);
         if (i >= a.Lq) continue;
         const int64_t at = (((int64_t)b * a.Lq + i) * a.H + h) * I::ROW;
 #pragma unroll
-        for (int db = 0; db < I::DB; ++db) {
-            const f32x4 x = none ? f32x4{0.f, 0.f, 0.f, 0.f} : o[nb][db] * inv;
-            store4<DT>(a.out + at + (16 * db + 4 * g) * I::EB, x);
-            if constexpr (DT != 0) {
-                if (a.rest) {
-                    f32x4 y;
-#pragma unroll
-                    for (int r = 0; r < 4; r += 2) {
-                        const unsigned w = seq_pack<DT>(x[r], x[r + 1]);
-                        y[r] = x[r] - seq_lo<DT>(w);
-                        y[r + 1] = x[r + 1] - seq_hi<DT>(w);
-                    }
-                    store4<DT>(a.rest + at + (16 * db + 4 * g) * I::EB, y);
-                }
-            }
+        for (int db = 0; db < I::DB; ++db) store_out<DT>(a, at + (16 * db + 4 * g) * I::EB, none ? f32x4{0.f, 0.f, 0.f, 0.f} : o[nb][db] * inv);
+    }
+}
+
+template <int DT, int D, int NB>
+__global__ __launch_bounds__(kBlock, 2) void band_fwd_kernel(BandArgs a) {
+    constexpr int STAGE = 2 * key_tile(DT) * Img<DT, D>::ROW;
+    __shared__ __attribute__((aligned(256))) unsigned char mem[stages(STAGE) * STAGE];
+    band_fwd<DT, D, NB, key_tile(DT)>(a, mem);
+}
+
+// The pieces of every row joined, in their order, four values a lane.
+template <int DT, int D>
+__global__ __launch_bounds__(kBlock) void band_join_kernel(BandArgs a) {
+    constexpr int LANES = D / 4;
+    const int64_t row = ((int64_t)blockIdx.x * kBlock + threadIdx.x) / LANES;   // (batch, head, query up to the pitch)
+    const int c = threadIdx.x % LANES, i = (int)(row % a.Lp);
+    const int64_t bh = row / a.Lp;
+    if (bh >= (int64_t)a.B * a.H) return;
+    const int b = (int)(bh / a.H), h = (int)(bh % a.H);
+    float top = -INFINITY, sum = 0.f;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (i < a.m(b)) {
+        const int64_t at = (bh * a.Lq + i) * a.fwd_splits;
+        for (int s = 0; s < a.fwd_splits; ++s) {
+            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (at + s));
+            const f32x4 o = *reinterpret_cast<const f32x4*>(a.part + (at + s) * D + 4 * c);
+            const float up = fmaxf(top, ml.x), ref = up == -INFINITY ? 0.f : up, f0 = seq_exp2(top - ref), f1 = seq_exp2(ml.x - ref);
+            sum = sum * f0 + ml.y * f1;
+            x = x * f0 + o * f1;
+            top = up;
         }
     }
+    if (c == 0 && a.lse) a.lse[row] = sum == 0.f ? INFINITY : top + __log2f(sum);
+    if (i < a.Lq) store_out<DT>(a, (((int64_t)b * a.Lq + i) * a.H + h) * Img<DT, D>::ROW + c * 4 * SeqT<DT>::bytes, sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : x * (1.f / sum));
 }
 
 // ====================================================================================================================================
 // gradients
 // ====================================================================================================================================
-// delta_i = do_i o_i, a row by the lanes that hold 16 bytes of it each.  16-bit: o is the stored output and the rest its rounding took, so
+// -delta_i = -do_i o_i (where the sums of do_i v_j start), a row by the lanes that hold 16 bytes of it each.  16-bit: o is the stored output and the rest its rounding took, so
 // that delta -- which is subtracted from every do_i v_j of the row -- is as good as from the 32-bit output.
 template <int DT, int D>
 __global__ __launch_bounds__(kBlock) void band_delta_kernel(BandArgs a) {
@@ -365,14 +462,14 @@ __global__ __launch_bounds__(kBlock) void band_delta_kernel(BandArgs a) {
     }
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1) d += __shfl_xor(d, o, 64);
-    if (c == 0) a.delta[((int64_t)b * a.H + h) * a.Lp + i] = d;
+    if (c == 0) a.delta[((int64_t)b * a.H + h) * a.Lp + i] = -d;
 }
 
 // dq: query-owning, streams k (both ways) and v (rows).  Tiles are taken 32 keys at a time.
 template <int DT, int D, int NB, int TB>
 __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, int group) {
     typedef Img<DT, D> I;
-    constexpr int ROWS = 16 * NB * kWaves, BYTES = TB * I::ROW;
+    constexpr int ROWS = 16 * NB * kWaves, BYTES = TB * I::ROW, STG = stages(2 * BYTES);
     auto lds = reinterpret_cast<unsigned char (*)[2][BYTES]>(mem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
     const int bh = spread_heads(group % (a.B * a.H), a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.kv);
@@ -403,22 +500,21 @@ __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, i
         }
         const unsigned char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
         const int pw0 = iw + shift, pw1 = min(iw + 16 * NB, m) - 1 + shift;
-        Stage<DT, D, TB> sk, sv;
-        if (kt.count) {
-            sk.load(kp, a.kl, kt.tile(0) * TB, n);
-            sv.load(vp, a.vl, kt.tile(0) * TB, n);
-            sk.store(lds[0][0]);
-            sv.store(lds[0][1]);
-        }
-        __syncthreads();
+        const Dma<DT, D, TB> dk(kp, a.kl, wave, lane), dv(vp, a.vl, wave, lane);
+        auto issue = [&](int t) {
+            const int row0 = kt.tile(t) * TB, st = t % STG;
+            dk.issue(lds[st][0], wave, row0, n);
+            dv.issue(lds[st][1], wave, row0, n);
+        };
+#pragma unroll
+        for (int t = 0; t < STG - 1; ++t)
+            if (t < kt.count) issue(t);
         for (int t = 0; t < kt.count; ++t) {
-            const unsigned char *ki = lds[t & 1][0], *vi = lds[t & 1][1];
+            const unsigned char *ki = lds[t % STG][0], *vi = lds[t % STG][1];
             const int j0 = kt.tile(t) * TB;
-            const bool more = t + 1 < kt.count;
-            if (more) {
-                sk.load(kp, a.kl, kt.tile(t + 1) * TB, n);
-                sv.load(vp, a.vl, kt.tile(t + 1) * TB, n);
-            }
+            if (STG == 3 && t + 1 < kt.count) landed<2 * Dma<DT, D, TB>::N>();
+            else landed<0>();
+            if (t + STG - 1 < kt.count) issue(t + STG - 1);
             if (iw < m && !a.none_sees(pw0, pw1, j0, j0 + TB - 1)) {
                 const bool part = j0 + TB > n || !a.all_see(pw0, pw1, j0, j0 + TB - 1);
 #pragma unroll
@@ -427,7 +523,10 @@ __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, i
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) s[nb][u] = z[nb][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        for (int nb = 0; nb < NB; ++nb) {   // (the second product's sum starts at -delta)
+                            s[nb][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                            z[nb][u] = f32x4{delta[nb], delta[nb], delta[nb], delta[nb]};
+                        }
 #pragma unroll
                         for (int ks = 0; ks < I::KS; ++ks) {
                             const Frag<DT> kf = I::row_frag(ki, 32 * kk + 16 * u + n16, ks, g), vf = I::row_frag(vi, 32 * kk + 16 * u + n16, ks, g);
@@ -438,17 +537,33 @@ __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, i
                             }
                         }
                     }
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) s[nb][u][r] = seq_exp2(fmaf(s[nb][u][r], a.c2, -lse[nb]));
+                    if (part) {
+                        const bool firsts = j0 < a.sinks;
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const Range r = keys_of(a, iw + 16 * nb + n16 + shift, n);
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const int j = j0 + 4 * g + 32 * kk + 16 * u + e;
+                                    s[nb][u][e] = r.in(j) | (firsts & (j < r.first)) ? s[nb][u][e] : 0.f;
+                                }
+                        }
+                    }
                     Frag<DT> zf[NB];
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                float p = seq_exp2(fmaf(s[nb][u][r], a.c2, -lse[nb]));
-                                if (part) p = a.sees(iw + 16 * nb + n16 + shift, j0 + 32 * kk + 16 * u + 4 * g + r, n) ? p : 0.f;
-                                z[nb][u][r] = p * (z[nb][u][r] - delta[nb]);
-                            }
+                            for (int r = 0; r < 4; ++r) z[nb][u][r] *= s[nb][u][r];
                         if constexpr (DT == 2) {
                             float mx = 0.f;
 #pragma unroll
@@ -462,18 +577,16 @@ __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, i
                         zf[nb] = as_frag<DT>(z[nb][0], z[nb][1]);
                     }
 #pragma unroll
-                    for (int db = 0; db < I::DB; ++db) {
-                        const Frag<DT> kf = I::col_frag(ki, 32 * kk, db, n16, g);
+                    for (int d0 = 0; d0 < I::DB; d0 += I::DN) {
+                        Frag<DT> kf[I::DN];
+                        I::col_frags(kf, ki, 32 * kk, d0, n16, g);
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) acc[nb][db] = seq_mma<DT>(kf, zf[nb], acc[nb][db]);
+                        for (int db = 0; db < I::DN; ++db)
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) acc[nb][d0 + db] = seq_mma<DT>(kf[db], zf[nb], acc[nb][d0 + db]);
                     }
                 }
             }
-            if (more) {
-                sk.store(lds[(t + 1) & 1][0]);
-                sv.store(lds[(t + 1) & 1][1]);
-            }
-            __syncthreads();
         }
     }
 #pragma unroll
@@ -504,9 +617,9 @@ struct KeyItem {
 template <int DT, int D, int NB, int TB>
 __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, int group) {
     typedef Img<DT, D> I;
-    constexpr int ROWS = 16 * NB * kWaves, BYTES = TB * I::ROW;
+    constexpr int ROWS = 16 * NB * kWaves, BYTES = TB * I::ROW, STG = stages(2 * BYTES);
     auto lds = reinterpret_cast<unsigned char (*)[2][BYTES]>(mem);
-    auto row_c = reinterpret_cast<float (*)[2][TB]>(mem + 4 * BYTES);   // lse, delta of the tile's queries
+    auto row_c = reinterpret_cast<float (*)[4][64]>(mem + STG * 2 * BYTES);   // lse, -delta of the tile's queries (and what waves 2, 3 fetch)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
     const int bk = spread_heads(group % (a.B * a.kv), a.B * a.kv), b = bk / a.kv, hk = bk % a.kv, G = a.H / a.kv, item = group / (a.B * a.kv);
     const KeyItem it(a, item);
@@ -534,29 +647,33 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
         Frag<DT> kf[NB][I::KS], vf[NB][I::KS];
         owner_frags<DT, D, NB>(kf, a.k + b * a.kb + hk * a.kh, a.kl, jw, n, n16, g, a.flip);
         owner_frags<DT, D, NB>(vf, a.v + b * a.vb + hk * a.vh, a.vl, jw, n, n16, g, 0u);
-        const int jw1 = min(jw + 16 * NB, n) - 1;
-        Stage<DT, D, TB> sq, sg;
-        float rc = 0.f;
-        auto load = [&](int u) {
-            const int h = hk * G + u / tiles, i0 = (first + u % tiles) * TB;
-            sq.load(a.q + b * a.qb + h * a.qh, a.ql, i0, m);
-            sg.load(a.go + b * a.gb + h * a.gh, a.gl, i0, m);
-            if (tid < 2 * TB) rc = (tid < TB ? a.lse : a.delta)[((int64_t)b * a.H + h) * a.Lp + i0 + tid % TB];
+        const int jw1 = min(jw + 16 * NB, n) - 1, h0 = hk * G;
+        Dma<DT, D, TB> dq(a.q + b * a.qb + h0 * a.qh, a.ql, wave, lane), dg(a.go + b * a.gb + h0 * a.gh, a.gl, wave, lane);
+        int ahead_h = u0 / tiles, ahead = u0 % tiles, now = ahead;   // head and tile of the next request, tile being worked on
+        const float* consts = (wave & 1 ? a.delta : a.lse) + ((int64_t)b * a.H + h0) * a.Lp;
+        const unsigned char *q0 = dq.base, *g0 = dg.base;
+        auto issue = [&](int st) {
+            const int i0 = (first + ahead) * TB;
+            dq.base = q0 + ahead_h * a.qh;
+            dg.base = g0 + ahead_h * a.gh;
+            dq.issue(lds[st][0], wave, i0, m);
+            dg.issue(lds[st][1], wave, i0, m);
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(consts + (int64_t)ahead_h * a.Lp + i0), 0, (a.Lp - i0) * 4, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(&row_c[st][wave][0]), 4, lane * 4, 0, 0, 0);
+            if (++ahead == tiles) { ahead = 0; ++ahead_h; }
         };
-        auto store = [&](int buf) {
-            sq.store(lds[buf][0]);
-            sg.store(lds[buf][1]);
-            if (tid < 2 * TB) row_c[buf][tid / TB][tid % TB] = rc;
-        };
-        load(u0);
-        store(0);
-        __syncthreads();
-        for (int u = u0; u < u1; ++u) {
-            const int buf = (u - u0) & 1;
+        const int count = u1 - u0;
+#pragma unroll
+        for (int t = 0; t < STG - 1; ++t)
+            if (t < count) issue(t);
+        for (int t = 0; t < count; ++t) {
+            const int buf = t % STG;
             const unsigned char *qi = lds[buf][0], *gi = lds[buf][1];
-            const int p0 = (first + u % tiles) * TB + shift, p1 = p0 + TB - 1;   // (queries behind m: do = 0 and P = 0)
-            const bool more = u + 1 < u1;
-            if (more) load(u + 1);
+            const int p0 = (first + now) * TB + shift, p1 = p0 + TB - 1;   // (queries behind m: do = 0 and P = 0)
+            if (++now == tiles) now = 0;
+            if (STG == 3 && t + 1 < count) landed<2 * Dma<DT, D, TB>::N + 1>();
+            else landed<0>();
+            if (t + STG - 1 < count) issue((t + STG - 1) % STG);
             if (jw < n && !a.none_sees(p0, p1, jw, jw1)) {
                 const bool part = !a.all_see(p0, p1, jw, jw1);
 #pragma unroll
@@ -564,8 +681,12 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
                     f32x4 s[NB][2], z[NB][2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
+                        const f32x4 del = *reinterpret_cast<const f32x4*>(&row_c[buf][1][32 * kk + 16 * x + 4 * g]);   // (-delta)
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) s[nb][x] = z[nb][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        for (int nb = 0; nb < NB; ++nb) {
+                            s[nb][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+                            z[nb][x] = del;
+                        }
 #pragma unroll
                         for (int ks = 0; ks < I::KS; ++ks) {
                             const Frag<DT> qf = I::row_frag(qi, 32 * kk + 16 * x + n16, ks, g), gf = I::row_frag(gi, 32 * kk + 16 * x + n16, ks, g);
@@ -576,21 +697,29 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
                             }
                         }
                     }
-                    Frag<DT> pf[NB], zf[NB];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const f32x4 lse = *reinterpret_cast<const f32x4*>(&row_c[buf][0][32 * kk + 16 * x + 4 * g]);
-                        const f32x4 del = *reinterpret_cast<const f32x4*>(&row_c[buf][1][32 * kk + 16 * x + 4 * g]);
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                float p = seq_exp2(fmaf(s[nb][x][r], a.c2, -lse[r]));
-                                if (part) p = a.sees(p0 + 32 * kk + 16 * x + 4 * g + r, jw + 16 * nb + n16, n) ? p : 0.f;
-                                s[nb][x][r] = p;
-                                z[nb][x][r] = p * (z[nb][x][r] - del[r]);
-                            }
+                            for (int r = 0; r < 4; ++r) s[nb][x][r] = seq_exp2(fmaf(s[nb][x][r], a.c2, -lse[r]));
                     }
+                    if (part) {
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const Range r = queries_of(a, jw + 16 * nb + n16);
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) s[nb][x][e] = r.in(p0 + 4 * g + 32 * kk + 16 * x + e) ? s[nb][x][e] : 0.f;
+                        }
+                    }
+                    Frag<DT> pf[NB], zf[NB];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) z[nb][x] *= s[nb][x];
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         if constexpr (DT == 2) {
@@ -609,18 +738,20 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
                         zf[nb] = as_frag<DT>(z[nb][0], z[nb][1]);
                     }
 #pragma unroll
-                    for (int db = 0; db < I::DB; ++db) {
-                        const Frag<DT> gf = I::col_frag(gi, 32 * kk, db, n16, g), qf = I::col_frag(qi, 32 * kk, db, n16, g);
+                    for (int d0 = 0; d0 < I::DB; d0 += I::DN) {
+                        Frag<DT> gf[I::DN], qf[I::DN];
+                        I::col_frags(gf, gi, 32 * kk, d0, n16, g);
+                        I::col_frags(qf, qi, 32 * kk, d0, n16, g);
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            av[nb][db] = seq_mma<DT>(gf, pf[nb], av[nb][db]);
-                            ak[nb][db] = seq_mma<DT>(qf, zf[nb], ak[nb][db]);
-                        }
+                        for (int db = 0; db < I::DN; ++db)
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                av[nb][d0 + db] = seq_mma<DT>(gf[db], pf[nb], av[nb][d0 + db]);
+                                ak[nb][d0 + db] = seq_mma<DT>(qf[db], zf[nb], ak[nb][d0 + db]);
+                            }
                     }
                 }
             }
-            if (more) store(buf ^ 1);
-            __syncthreads();
         }
     }
 #pragma unroll
@@ -651,11 +782,12 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
 
 // Both in one launch, the key blocks first: either alone would leave compute units empty at the sizes where time counts, and at its end.
 template <int DT, int D> constexpr int bwd_bytes() {
-    constexpr int q = 4 * key_tile(DT) * Img<DT, D>::ROW, k = 4 * query_tile(DT, D) * Img<DT, D>::ROW + 16 * query_tile(DT, D);
+    constexpr int qs = 2 * key_tile(DT) * Img<DT, D>::ROW, ks = 2 * query_tile(DT, D) * Img<DT, D>::ROW;
+    constexpr int q = stages(qs) * qs, k = stages(ks) * (ks + 1024);
     return q > k ? q : k;
 }
 template <int DT, int D, int NB>
-__global__ __launch_bounds__(kBlock, D == 128 && DT != 0 ? 1 : 2) void band_bwd_kernel(BandArgs a) {
+__global__ __launch_bounds__(kBlock, 2) void band_bwd_kernel(BandArgs a) {
     __shared__ __attribute__((aligned(256))) unsigned char mem[bwd_bytes<DT, D>()];
     if ((int)blockIdx.x < a.key_groups) band_dkv<DT, D, NB, query_tile(DT, D)>(a, mem, blockIdx.x);
     else band_dq<DT, D, NB, key_tile(DT)>(a, mem, blockIdx.x - a.key_groups);
@@ -683,34 +815,68 @@ __global__ __launch_bounds__(kBlock) void band_sum_kernel(BandArgs a, int items,
 // ====================================================================================================================================
 // host side
 // ====================================================================================================================================
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t reach(const ix_band* s) {   // rows on both sides that a band takes from a row's place
+    const int64_t far = s->window > 0 ? s->window - 1 : (int64_t)s->Lq + s->Lk;
+    return s->causal ? far : 2 * far;
+}
+
+// Owner rows: 64 or 128 a workgroup (one or two blocks of 16 for every wave).  Two blocks read LDS half as often for the same products, one
+// gives twice as many workgroups and waves.  Measured, bf16 (us, one / two): forward head dim 64, 64 workgroups of 128 rows 9 / 13, 272 of
+// them 24 / 28, 800 of them 120 / 105; head dim 32, 544: 27 / 30, 1 024: 142 / 132; head dim 128, where LDS counts double, 64: 14 / 18,
+// 512: 66 / 57, 2 048: 399 / 310.  Gradients head dim 64, 192: 12.6 / 15, 576: 49 / 49, 1 632: 322 / 284; head dim 128 only one (two take
+// the registers of a second wave: 20 / 37 at 176, 667 / 913 at 2 048).  f32 has room for one.
+int fwd_nb(const ix_band* s) {
+    if (s->dtype == 0) return 1;
+    return (int64_t)s->batch * s->heads * div_up(s->Lq, 128) < (s->hd == 128 ? 256 : 600) ? 1 : 2;
+}
+int bwd_nb(const ix_band* s) {
+    if (s->dtype == 0 || s->hd == 128) return 1;
+    return (int64_t)s->batch * (s->heads * div_up(s->Lq, 128) + s->kv_heads * div_up(s->Lk, 128)) < 600 ? 1 : 2;
+}
+
+// Pieces of the forward's key tiles: where the rows are so few that half of the compute units would stand idle, up to 32 pieces of at least
+// four tiles (40 queries of 16 heads over 6 000 keys: 101 us in one piece).
+int fwd_splits(const ix_band* s) {
+    const int64_t groups = (int64_t)s->batch * s->heads * div_up(s->Lq, owner_rows(fwd_nb(s)));
+    if (groups > 128) return 1;
+    const int tb = key_tile(s->dtype);
+    const int64_t all = div_up(s->Lk, tb), some = div_up(reach(s) + 64, tb) + 1 + div_up(s->sinks, tb), tiles = some < all ? some : all;
+    int64_t r = 512 / groups;
+    if (r > tiles / 4) r = tiles / 4;
+    return (int)(r < 2 ? 1 : r > 32 ? 32 : r);
+}
+size_t fwd_part(const ix_band* s) {   // partial rows
+    const int r = fwd_splits(s);
+    return r == 1 ? 0 : (size_t)s->batch * s->heads * s->Lq * r;
+}
+
 struct KeyPlan { int blocks, wide, wide_splits, splits, items; };
 
 // Splits of dk / dv.  A block of keys streams the queries of its band; a block with some of the first `sinks` keys streams all of them, and
-// would run long after the others: it is cut into pieces of about the others' length.  Where all blocks together are fewer than the
-// compute units (few key heads, many query heads), every block is cut until they are not.
+// where these are more than two and a half times the others' it would run on alone: it is cut into pieces of up to twice the others'
+// length.  Where all blocks together are fewer than the compute units (few key heads, many query heads), every block is cut.
 KeyPlan key_plan(const ix_band* s) {
     KeyPlan r;
-    const int rows = owner_rows(s->dtype), group = s->heads / s->kv_heads;
-    r.blocks = (s->Lk + rows - 1) / rows;
-    r.wide = s->sinks > 0 ? (s->sinks < s->Lk ? (s->sinks + rows - 1) / rows : r.blocks) : 0;
-    const int64_t far = s->window > 0 ? s->window : (int64_t)s->Lq + s->Lk;
-    const int tb = query_tile(s->dtype, s->hd);
-    const int64_t all = (s->Lq + tb - 1) / tb, band = ((s->causal ? far : 2 * far) + rows + tb - 1) / tb + 1, each = (band < all ? band : all) * group;
+    const int rows = owner_rows(bwd_nb(s)), group = s->heads / s->kv_heads, tb = query_tile(s->dtype, s->hd);
+    r.blocks = (int)div_up(s->Lk, rows);
+    r.wide = s->sinks > 0 ? (s->sinks < s->Lk ? (int)div_up(s->sinks, rows) : r.blocks) : 0;
+    const int64_t all = div_up(s->Lq, tb), band = div_up(reach(s) + rows, tb) + 1, each = (band < all ? band : all) * group;
     const int64_t wgs = (int64_t)s->batch * s->kv_heads * r.blocks;
-    int64_t sp = wgs < 256 ? (256 + wgs - 1) / wgs : 1;
-    if (sp > (each + 3) / 4) sp = (each + 3) / 4;   // (no piece under four tiles)
+    int64_t sp = wgs < 256 ? div_up(256, wgs) : 1;
+    if (sp > div_up(each, 4)) sp = div_up(each, 4);   // (no piece under four tiles)
     r.splits = (int)(sp < 1 ? 1 : sp);
-    const int64_t piece = (each + r.splits - 1) / r.splits;
-    int64_t ws = (all * group + piece - 1) / piece;
-    if (ws > 64) ws = 64;
-    r.wide_splits = (int)(ws < 1 ? 1 : ws);
+    const int64_t piece = div_up(each, r.splits);
+    int64_t ws = 2 * all * group <= 5 * piece ? 1 : div_up(all * group, 2 * piece);
+    if (r.splits > 1 && ws < r.splits) ws = r.splits;
+    r.wide_splits = (int)(ws > 64 ? 64 : ws);
     r.items = r.wide * r.wide_splits + (r.blocks - r.wide) * r.splits;
     return r;
 }
 
 size_t part_bytes(const ix_band* s, const KeyPlan& r) {
     if (r.splits == 1 && (r.wide_splits == 1 || r.wide == 0)) return 0;
-    return (size_t)s->batch * s->kv_heads * r.items * 2 * owner_rows(s->dtype) * s->hd * 4;
+    return (size_t)s->batch * s->kv_heads * r.items * 2 * owner_rows(bwd_nb(s)) * s->hd * 4;
 }
 
 int64_t lse_pitch(const ix_band* s) { return ((int64_t)s->Lq + 127) / 128 * 128; }
@@ -729,6 +895,7 @@ int band_of(BandArgs& a, const ix_band* s, const char* who) {
     const int64_t eb = s->dtype == 0 ? 4 : 2;
     for (int64_t x : {s->q_sb, s->q_sl, s->q_sh, s->k_sb, s->k_sl, s->k_sh, s->v_sb, s->v_sl, s->v_sh})
         IX_CHECK_ARG(x * eb % 16 == 0, "%s: rows that do not start on 16 bytes", who);
+    for (int64_t x : {s->q_sl, s->k_sl, s->v_sl}) IX_CHECK_ARG(x >= 0 && x * eb < (1 << 24), "%s: rows 2^24 bytes apart or more", who);
     a = BandArgs{};
     a.q = static_cast<const unsigned char*>(s->q);
     a.k = static_cast<const unsigned char*>(s->k);
@@ -752,22 +919,57 @@ int band_of(BandArgs& a, const ix_band* s, const char* who) {
     return IX_OK;
 }
 
+template <int DT, int D> void launch_fwd(const BandArgs& a, int nb, dim3 grid, hipStream_t stream) {
+    if constexpr (DT == 0) band_fwd_kernel<DT, D, 1><<<grid, kBlock, 0, stream>>>(a);
+    else if (nb == 1) band_fwd_kernel<DT, D, 1><<<grid, kBlock, 0, stream>>>(a);
+    else band_fwd_kernel<DT, D, 2><<<grid, kBlock, 0, stream>>>(a);
+}
+template <int DT, int D> void launch_bwd(const BandArgs& a, int nb, unsigned groups, hipStream_t stream) {
+    if constexpr (DT == 0) band_bwd_kernel<DT, D, 1><<<groups, kBlock, 0, stream>>>(a);
+    else if constexpr (D == 128) band_bwd_kernel<DT, D, 1><<<groups, kBlock, 0, stream>>>(a);
+    else if (nb == 1) band_bwd_kernel<DT, D, 1><<<groups, kBlock, 0, stream>>>(a);
+    else band_bwd_kernel<DT, D, 2><<<groups, kBlock, 0, stream>>>(a);
+}
+
 }  // namespace
 
-#define BAND_HD(CALL, DT) { if (s->hd == 32) CALL(DT, 32); else if (s->hd == 64) CALL(DT, 64); else CALL(DT, 128); }
+#define BAND_HD(CALL, DT) { if (s->hd == 32) { CALL(DT, 32); } else if (s->hd == 64) { CALL(DT, 64); } else { CALL(DT, 128); } }
 #define BAND_GO(CALL) { if (s->dtype == 0) BAND_HD(CALL, 0) else if (s->dtype == 1) BAND_HD(CALL, 1) else BAND_HD(CALL, 2) }
 
-extern "C" int ix_band_attn_fwd(const struct ix_band* s, void* out, float* lse, void* rest, hipStream_t stream) {
+extern "C" int ix_workspace_bytes_band_attn_fwd(const struct ix_band* s, size_t* out_host) {
+    BandArgs a;
+    if (int rc = band_of(a, s, "ix_workspace_bytes_band_attn_fwd")) return rc;
+    IX_CHECK_ARG(out_host, "ix_workspace_bytes_band_attn_fwd: null output");
+    *out_host = fwd_part(s) * (s->hd + 2) * 4;
+    return IX_OK;
+}
+
+extern "C" int ix_band_attn_fwd(const struct ix_band* s, void* out, float* lse, void* rest, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     BandArgs a;
     if (int rc = band_of(a, s, "ix_band_attn_fwd")) return rc;
     IX_CHECK_ARG(out && ix_al16(out) && ix_al16(rest), "ix_band_attn_fwd: null or unaligned output");
+    const size_t parts = fwd_part(s), need = parts * (s->hd + 2) * 4;
+    if (need && (!workspace || workspace_bytes < need || !ix_al16(workspace))) {
+        ix_set_error("ix_band_attn_fwd: workspace of %zu bytes (16-byte aligned), %zu needed", workspace ? workspace_bytes : (size_t)0, need);
+        return IX_ERR_WORKSPACE;
+    }
     a.out = static_cast<unsigned char*>(out);
     a.rest = s->dtype ? static_cast<unsigned char*>(rest) : nullptr;
     a.lse = lse;
-    const dim3 grid(a.B * a.H, (a.Lq + owner_rows(s->dtype) - 1) / owner_rows(s->dtype));
-#define BAND_FWD(DT, D) band_fwd_kernel<DT, D, owner_blocks(DT), key_tile(DT)><<<grid, kBlock, 0, stream>>>(a)
+    a.fwd_splits = fwd_splits(s);
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = a.part + parts * s->hd;
+    const int nb = fwd_nb(s), rows = owner_rows(nb);
+    const dim3 grid(a.B * a.H, (a.Lq + rows - 1) / rows, a.fwd_splits);
+#define BAND_FWD(DT, D) launch_fwd<DT, D>(a, nb, grid, stream)
     BAND_GO(BAND_FWD)
     IX_CHECK_LAUNCH("ix_band_attn_fwd");
+    if (a.fwd_splits > 1) {
+        const unsigned groups = (unsigned)div_up((int64_t)a.B * a.H * a.Lp * (s->hd / 4), kBlock);
+#define BAND_JOIN(DT, D) band_join_kernel<DT, D><<<groups, kBlock, 0, stream>>>(a)
+        BAND_GO(BAND_JOIN)
+        IX_CHECK_LAUNCH("ix_band_attn_fwd (join)");
+    }
     return IX_OK;
 }
 
@@ -795,6 +997,7 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
     IX_CHECK_ARG(out && (rest || s->dtype == 0) && lse && d_out && dq && dk && dv, "ix_band_attn_bwd: null pointer");
     IX_CHECK_ARG(ix_al16(out) && ix_al16(rest) && ix_al16(d_out) && ix_al16(dq) && ix_al16(dk) && ix_al16(dv), "ix_band_attn_bwd: unaligned pointer");
     for (int64_t x : {g_sb, g_sl, g_sh}) IX_CHECK_ARG(x * eb % 16 == 0, "ix_band_attn_bwd: rows that do not start on 16 bytes");
+    IX_CHECK_ARG(g_sl >= 0 && g_sl * eb < (1 << 24), "ix_band_attn_bwd: rows 2^24 bytes apart or more");
     const KeyPlan r = key_plan(s);
     const size_t parts = part_bytes(s, r), need = (size_t)a.B * a.H * a.Lp * 4 + parts;
     if (!workspace || workspace_bytes < need || !ix_al16(workspace)) {
@@ -814,7 +1017,7 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
     a.wide_blocks = r.wide;
     a.wide_splits = r.wide_splits;
     a.splits = r.splits;
-    const int rows = owner_rows(s->dtype);
+    const int nb = bwd_nb(s), rows = owner_rows(nb);
     const int64_t key_groups = (int64_t)a.B * a.kv * r.items, groups = key_groups + (int64_t)a.B * a.H * ((a.Lq + rows - 1) / rows);
     const int64_t delta_groups = ((int64_t)a.B * a.H * a.Lp * (s->hd * eb / 16) + kBlock - 1) / kBlock;
     IX_CHECK_ARG(groups < (1ll << 31) && delta_groups < (1ll << 31), "ix_band_attn_bwd: too many rows for one launch");
@@ -822,14 +1025,14 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
 #define BAND_DELTA(DT, D) band_delta_kernel<DT, D><<<(unsigned)delta_groups, kBlock, 0, stream>>>(a)
     BAND_GO(BAND_DELTA)
     IX_CHECK_LAUNCH("ix_band_attn_bwd (delta)");
-#define BAND_BWD(DT, D) band_bwd_kernel<DT, D, owner_blocks(DT)><<<(unsigned)groups, kBlock, 0, stream>>>(a)
+#define BAND_BWD(DT, D) launch_bwd<DT, D>(a, nb, (unsigned)groups, stream)
     BAND_GO(BAND_BWD)
     IX_CHECK_LAUNCH("ix_band_attn_bwd");
     if (parts) {
         const int blocks = r.splits > 1 ? r.blocks : r.wide;
         IX_CHECK_ARG(blocks <= 65535, "ix_band_attn_bwd: too many keys for one launch");
         const dim3 sgrid(a.B * a.kv, blocks, 4);
-#define BAND_SUM(DT, D) band_sum_kernel<DT, D><<<sgrid, kBlock, 0, stream>>>(a, r.items, owner_rows(DT))
+#define BAND_SUM(DT, D) band_sum_kernel<DT, D><<<sgrid, kBlock, 0, stream>>>(a, r.items, rows)
         BAND_GO(BAND_SUM)
         IX_CHECK_LAUNCH("ix_band_attn_bwd (sum)");
     }

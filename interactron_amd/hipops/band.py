@@ -25,10 +25,10 @@ _NAMES = ("q", "k", "v", "q_lens", "kv_lens")
 
 
 def _dense_rows(t):
-    """t, or a copy whose rows the kernels can read: last dimension dense, every row on 16 bytes"""
+    """t, or a copy whose rows the kernels can read: last dimension dense, every row on 16 bytes and less than 2^24 bytes from the next"""
     per = 16 // t.element_size()
     sb, sl, sh, sd = t.stride()
-    if sd != 1 or sb % per or sl % per or sh % per or t.data_ptr() & 15:
+    if sd != 1 or sb % per or sl % per or sh % per or t.data_ptr() & 15 or sl >= per << 20:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -69,7 +69,11 @@ class BandAttention(Function):
                 rest = torch.empty(shape, dtype=q.dtype, device=q.device)
             ctx.how = (window, sinks, causal, scale)
             ctx.save_for_backward(q, k, v, out, lse, rest, q_lens, kv_lens)
-        rc = _L().ix_band_attn_fwd(ctypes.byref(band), out.data_ptr(), _ptr(lse), _ptr(rest), s)
+        ref, n, ws = ctypes.byref(band), ctypes.c_size_t(0), None
+        _chk(_L().ix_workspace_bytes_band_attn_fwd(ref, ctypes.byref(n)), "ix_workspace_bytes_band_attn_fwd")
+        if n.value:
+            ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+        rc = _L().ix_band_attn_fwd(ref, out.data_ptr(), _ptr(lse), _ptr(rest), _ptr(ws), n.value, s)
         if rc:
             _chk(rc, "ix_band_attn_fwd")
         return out

@@ -50,7 +50,7 @@ def c_band(**change):
                                     dict(scale=float("inf")), dict(q_sl=252), dict(v_sh=33), dict(batch=1 << 29)], ids=str)
 def test_c_entries_refuse_a_bad_description(change):
     L, c, n = _lib.load(), c_band(**change), ctypes.c_size_t(0)
-    for rc in (L.ix_band_attn_fwd(ctypes.byref(c), 4096, 4096, 4096, None), L.ix_workspace_bytes_band_attn_bwd(ctypes.byref(c), ctypes.byref(n)),
+    for rc in (L.ix_band_attn_fwd(ctypes.byref(c), 4096, 4096, 4096, 4096, 1 << 30, None), L.ix_workspace_bytes_band_attn_fwd(ctypes.byref(c), ctypes.byref(n)), L.ix_workspace_bytes_band_attn_bwd(ctypes.byref(c), ctypes.byref(n)),
                L.ix_band_attn_bwd(ctypes.byref(c), 4096, 4096, 4096, 4096, 1280, 256, 64, 4096, 4096, 4096, 4096, 1 << 30, None)):
         assert rc == -1 and L.ix_last_error()
 
@@ -58,13 +58,17 @@ def test_c_entries_refuse_a_bad_description(change):
 def test_c_entries_refuse_bad_buffers():
     L, c, n = _lib.load(), c_band(), ctypes.c_size_t(0)
     ref = ctypes.byref(c)
-    assert L.ix_band_attn_fwd(ref, None, None, None, None) == -1 and L.ix_band_attn_fwd(ref, 4104, None, None, None) == -1
-    assert L.ix_band_attn_fwd(ref, 4096, 4096, 4104, None) == -1
+    assert L.ix_band_attn_fwd(ref, None, None, None, None, 0, None) == -1 and L.ix_band_attn_fwd(ref, 4104, None, None, None, 0, None) == -1
+    assert L.ix_band_attn_fwd(ref, 4096, 4096, 4104, None, 0, None) == -1
     assert L.ix_workspace_bytes_band_attn_bwd(ref, ctypes.byref(n)) == 0 and n.value >= 2 * 4 * 128 * 4
     good = [ref, 4096, 4096, 4096, 4096, 1280, 256, 64, 4096, 4096, 4096, 4096, n.value, None]
     for place, value, code in ((1, None, -1), (2, None, -1), (3, None, -1), (4, 4104, -1), (6, 100, -1), (8, None, -1), (9, 4104, -1), (11, None, -3), (11, 4100, -3), (12, n.value - 1, -3)):
         args = list(good)
         args[place] = value
         assert L.ix_band_attn_bwd(*args) == code, (place, L.ix_last_error())
+    few = c_band(Lq=3, Lk=5000, q_sb=768, k_sb=640000, v_sb=640000)   # few rows over many keys: pieces
+    assert L.ix_workspace_bytes_band_attn_fwd(ctypes.byref(few), ctypes.byref(n)) == 0 and n.value >= 2 * 2 * 4 * 3 * 66 * 4
+    for ws, size in ((None, n.value), (4100, n.value), (4096, n.value - 1)):
+        assert L.ix_band_attn_fwd(ctypes.byref(few), 4096, None, None, ws, size, None) == -3
     p = ctypes.c_int64(0)
     assert L.ix_band_attn_lse_pitch(0, ctypes.byref(p)) == -1 and L.ix_band_attn_lse_pitch(129, ctypes.byref(p)) == 0 and p.value == 256

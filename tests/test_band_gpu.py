@@ -131,6 +131,17 @@ def test_long_rows_and_blocks_cut_into_splits(dtype, Lq, Lk, H, kv, window, sink
 
 
 @TYPES
+@pytest.mark.parametrize("Lq, Lk, how", [(1, 4000, {}), (3, 2500, dict(causal=False)), (70, 3000, dict(window=2000, sinks=130)), (40, 1200, dict(window=5, sinks=1000))])
+def test_few_queries_over_many_keys(dtype, Lq, Lk, how):
+    """pieces of the keys, joined; with gradients, and with a batch whose lengths leave pieces and rows empty"""
+    q, k, v, do = inputs(1, Lq, Lk, 4, 2, 64, dtype)
+    check(q, k, v, do, **how)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    q, k, v, do = inputs(3, Lq, Lk, 2, 1, 128, dtype)
+    check(q, k, v, do, q_lens=ints(Lq, Lq // 2, Lq), kv_lens=ints(Lk, 37, 0), **how)
+
+
+@TYPES
 def test_views(dtype):
     """a packed projection in place, rows off 16 bytes, swapped axes, inputs that are one row many times"""
     from interactron_amd import hipops
