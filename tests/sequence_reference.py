@@ -99,7 +99,10 @@ def band_attention(q, k, v, window, sinks, causal, scale=None, q_lens=None, kv_l
     names = ("out",) if do is None else ("out", "dq", "dk", "dv")
     shapes = dict(out=q.shape, dq=q.shape, dk=k.shape, dv=k.shape)
     val, err = ({x: np.zeros(shapes[x]) for x in names} for _ in range(2))
-    h = 0.0 if dtype == torch.float32 else half_step(dtype)   # the rounding of weights and of score gradients to the type
+    # 16-bit types: weights are rounded to the type (h), score gradients are carried as two of its terms (2 h^2), and the output that delta
+    # comes from as two terms too (fp16: the second no finer than 2^-25)
+    h = 0.0 if dtype == torch.float32 else half_step(dtype)
+    h_out, floor = (U, 0.0) if dtype == torch.float32 else (2 * h * h, 2.0 ** -25 if dtype == torch.float16 else 0.0)
     for b in range(B):
         m = Lq if q_lens is None else min(max(int(q_lens[b]), 0), Lq)
         n = Lk if kv_lens is None else min(max(int(kv_lens[b]), 0), Lk)
@@ -123,10 +126,9 @@ def band_attention(q, k, v, window, sinks, causal, scale=None, q_lens=None, kv_l
             g = do[b, :m, i]
             dp, delta = g @ vv.T, (g * o).sum(1, keepdims=True)
             ds = p * (dp - delta)
-            # delta comes from the output as it was stored (half a step of the type, 32-bit sums on top)
-            e_delta = (np.abs(g) * (half_step(dtype) * np.abs(o) + err["out"][b, :m, i] + (D + 2) * U * np.abs(o))).sum(1, keepdims=True)
+            e_delta = (np.abs(g) * (h_out * np.abs(o) + floor + err["out"][b, :m, i] + (D + 2) * U * np.abs(o))).sum(1, keepdims=True)
             e_dp = (D + 2) * U * (np.abs(g) @ np.abs(vv).T)
-            e_ds = np.abs(ds) * (rel + h + 4 * U) + p * (1 + rel) * (e_dp + e_delta)
+            e_ds = np.abs(ds) * (rel + 2 * h * h + 4 * U) + p * (1 + rel) * (e_dp + e_delta)
             if dtype == torch.float16:   # ... and score gradients are carried up to 2^15, weights up to 2^10
                 e_ds = e_ds + see * 2.0 ** -38 * np.abs(ds).max()
             val["dq"][b, :m, i] = scale * ds @ kk
