@@ -392,8 +392,8 @@ __device__ __forceinline__ unsigned weight_key(float w) {
 
 __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, const int* lens, int* kept, int* left, int kv, int cap, int budget,
                                                            int sinks, int recent) {
-    __shared__ unsigned hist[kSelWaves][256];
-    __shared__ unsigned total[256], pick[2];
+    // counts by pass, in four copies a quarter of the lanes each (on different banks): weights share few values of the first digit
+    __shared__ __attribute__((aligned(16))) unsigned hist[4][4][256 + 16];
     __shared__ int more[kSelWaves], same[kSelWaves];
     const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n = min(max(lens[b], 0), cap);
@@ -424,47 +424,47 @@ __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, 
     for (int i = tid; i < sinks; i += kSelBlock) out[i] = i;
     for (int i = tid; i < recent; i += kSelBlock) out[budget - recent + i] = m1 + i;
     if (need == 0) return;
+    for (int i = tid; i < 4 * 4 * 272; i += kSelBlock) (&hist[0][0][0])[i] = 0;
+    __syncthreads();
     unsigned prefix = 0, mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < kSelWaves * 256; i += kSelBlock) (&hist[0][0])[i] = 0;
-        __syncthreads();
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass) {
+        const int shift = 24 - 8 * pass;
+        unsigned* mine = hist[pass][lane & 3];
         for (int from = w0; from < w1; from += kPart) {
             if (!once) fetch(from);
 #pragma unroll
-            for (int u = 0; u < kSelHeld; ++u)
-                if (from + 64 * u + lane < w1 && (held[u] & mask) == prefix) atomicAdd(&hist[wave][(held[u] >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (tid < 256) {
-            unsigned s = 0;
-#pragma unroll
-            for (int k = 0; k < kSelWaves; ++k) s += hist[k][tid];
-            total[tid] = s;
-        }
-        __syncthreads();
-        if (wave == 0) {   // the digit at which the count from above reaches `need`: lane l holds digits 255 - 4 l down to 252 - 4 l
-            unsigned c[4], own = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) { c[k] = total[255 - 4 * lane - k]; own += c[k]; }
-            unsigned upto = own;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const unsigned x = __shfl_up(upto, o, 64);
-                if (lane >= o) upto += x;
-            }
-            unsigned before = upto - own;
-            if (before < need && need <= upto) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (before < need && need <= before + c[k]) { pick[0] = 255 - 4 * lane - k; pick[1] = need - before; }
-                    before += c[k];
-                }
+            for (int u = 0; u < kSelHeld; ++u) {
+                if (from + 64 * u >= w1) break;   // (uniform)
+                if (from + 64 * u + lane < w1 && (held[u] & mask) == prefix) atomicAdd(&mine[(held[u] >> shift) & 255], 1u);
             }
         }
-        __syncthreads();
-        prefix |= pick[0] << shift;
+        __syncthreads();   // (the only one of a pass: every wave finds the digit by itself)
+        // the digit at which the count from above reaches `need`: lane l holds digits 255 - 4 l down to 252 - 4 l
+        unsigned c[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(&hist[pass][k][252 - 4 * lane]);
+            c[0] += x.w; c[1] += x.z; c[2] += x.y; c[3] += x.x;
+        }
+        const unsigned own = c[0] + c[1] + c[2] + c[3];
+        unsigned upto = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned x = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += x;
+        }
+        unsigned before = upto - own, digit = 0, rest = 0;
+        const unsigned long long hit = __ballot(before < need && need <= upto);   // (one lane: at least `need` keys carry the prefix)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (before < need && need <= before + c[k]) { digit = 255 - 4 * lane - k; rest = need - before; }
+            before += c[k];
+        }
+        const int from = __ffsll((long long)hit) - 1;
+        prefix |= __builtin_amdgcn_readlane(digit, from) << shift;
+        need = __builtin_amdgcn_readlane(rest, from);
         mask |= 255u << shift;
-        need = pick[1];
     }
     // `prefix` is the smallest weight that stays, `need` of its equals stay with it
     int a = 0, e = 0;
@@ -472,6 +472,7 @@ __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, 
         if (!once) fetch(from);
 #pragma unroll
         for (int u = 0; u < kSelHeld; ++u) {
+            if (from + 64 * u >= w1) break;
             const bool in = from + 64 * u + lane < w1;
             a += __popcll(__ballot(in && held[u] > prefix));
             e += __popcll(__ballot(in && held[u] == prefix));
@@ -486,6 +487,7 @@ __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, 
         if (!once) fetch(from);
 #pragma unroll
         for (int u = 0; u < kSelHeld; ++u) {
+            if (from + 64 * u >= w1) break;
             const int i = from + 64 * u + lane;
             const unsigned long long equal = __ballot(i < w1 && held[u] == prefix);
             const bool stay = i < w1 && (held[u] > prefix || (held[u] == prefix && eq + __popcll(equal & below) < (int)need));
@@ -620,9 +622,11 @@ struct Plan {   // of one attention launch
     size_t o, ml, logits;   // floats
 };
 
-// Splits.  A cache of up to 32 tiles is one piece for eight waves: no join, one launch.  Longer ones are cut into about 1 024 workgroups of
-// four waves (two to four of them are resident on a compute unit), in pieces of at least one tile a wave, and of at most 512 keys where
-// several sequences of different lengths have to even out.
+// Splits.  A cache of up to 32 tiles is one piece for eight waves: no join, one launch.  Longer ones are cut into about 512 workgroups of
+// four waves (two are resident on a compute unit at head dim 128), or 1 024 where several sequences may differ in length; in pieces of at
+// least one tile a wave and at most 2 048 (1 024) keys.  A workgroup costs some microseconds before and after its keys, a rest of the
+// last round as much as a piece: 32 sequences of up to 8 192 tokens in pieces of 256 / 512 / 1 024 keys 125 / 111 / 111 us (join 8 / 7 / 6);
+// one of 131 071 tokens in 512 / 1 024 / 2 048 workgroups 94 / 96 / 99 us (join 5 / 7 / 14).
 Plan plan_of(const ix_paged_cache* s, int heads, int window, int sinks, int accumulate) {
     Plan r;
     r.kt = s->dtype == 0 ? 16 : 32;
@@ -642,8 +646,8 @@ Plan plan_of(const ix_paged_cache* s, int heads, int window, int sinks, int accu
     if (seen <= 32) {
         r.splits = 1;
     } else {
-        const int64_t most = (s->batch > 1 ? 512 : 2048) / r.kt;
-        int64_t per = rows * seen / 1024;
+        const int64_t most = (s->batch > 1 ? 1024 : 2048) / r.kt;
+        int64_t per = rows * seen / (s->batch > 1 ? 1024 : 512);
         if (per < r.least) per = r.least;
         if (per > most) per = rows * seen / most <= 65536 ? most : rows * seen / 65536;
         r.splits = (int)((seen + per - 1) / per);

@@ -62,11 +62,11 @@ class BandAttention(Function):
             return q.new_zeros(shape)
         q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
         band = _band(q, k, v, q_lens, kv_lens, window, sinks, causal, scale)
-        out, lse, rest = torch.empty(shape, dtype=q.dtype, device=q.device), None, None
+        out, lse, rest = q.new_empty(shape), None, None
         if recorded:   # the rows' normalisers and, with 16-bit types, what rounding took from the output: for the gradients
             lse = torch.empty(shape[0], shape[2], -(-shape[1] // 128) * 128, dtype=torch.float32, device=q.device)
             if q.dtype is not torch.float32:
-                rest = torch.empty(shape, dtype=q.dtype, device=q.device)
+                rest = q.new_empty(shape)
             ctx.how = (window, sinks, causal, scale)
             ctx.save_for_backward(q, k, v, out, lse, rest, q_lens, kv_lens)
         ref, n, ws = ctypes.byref(band), ctypes.c_size_t(0), None
@@ -94,7 +94,7 @@ class BandAttention(Function):
         n = ctypes.c_size_t(0)
         _chk(_L().ix_workspace_bytes_band_attn_bwd(band, ctypes.byref(n)), "ix_workspace_bytes_band_attn_bwd")
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        dq, dk, dv = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         gb, gl, gh, _ = do.stride()
         rc = _L().ix_band_attn_bwd(band, out.data_ptr(), _ptr(rest), lse.data_ptr(), do.data_ptr(), gb, gl, gh, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                    ws.data_ptr(), n.value, s)

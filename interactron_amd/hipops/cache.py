@@ -55,7 +55,7 @@ def _here(names, *ts):
 
 
 def _whole(t, name, dtype, shape):
-    if t.dtype != dtype or t.shape != shape:
+    if t.dtype is not dtype or t.shape != shape:
         raise ValueError("%s must be %s %s, got %s %s" % (name, dtype, list(shape), t.dtype, list(t.shape)))
     if not t.is_contiguous():
         raise ValueError("%s must be contiguous: it is used in place" % name)
@@ -77,33 +77,36 @@ class PagedCache:
     lens     int32 [batch]: tokens held
     weight   float32 [batch, kv_heads, pages * page] or None: the attention each token has had so far
     """
-    __slots__ = ("k", "v", "table", "lens", "weight", "kv_heads", "hd", "page", "batch", "pages", "capacity", "c", "ref")
+    __slots__ = ("k", "v", "table", "lens", "weight", "kv_heads", "hd", "page", "batch", "pages", "capacity", "dtype", "c", "ref")
 
     def __init__(self, k, v, table, lens, weight=None):
-        shape, code = k.shape, _DTYPES.get(k.dtype)
+        shape, dtype = k.shape, k.dtype
+        code = _DTYPES.get(dtype)
         if len(shape) != 4 or code is None:
-            raise ValueError("cache keys must be [pages_total, kv_heads, page, hd] in float32, bfloat16 or float16, got %s %s" % (k.dtype, list(shape)))
+            raise ValueError("cache keys must be [pages_total, kv_heads, page, hd] in float32, bfloat16 or float16, got %s %s" % (dtype, list(shape)))
         total, kv, page, hd = shape
         if hd not in _HEAD_DIMS:
             raise ValueError("a cache of head dim %d: %s are supported" % (hd, _HEAD_DIMS))
         if page not in _PAGES:
             raise ValueError("a page of %d tokens: powers of two from 16 to 1024 are supported" % page)
-        if table.dim() != 2 or not table.numel() or not k.numel():
+        if table.dim() != 2 or not table.numel() or not total or not kv:
             raise ValueError("an empty cache, or a page table that is not [batch, pages]: %s, %s" % (list(shape), list(table.shape)))
         B, pages = table.shape
-        _whole(k, "cache keys", k.dtype, shape)
-        _whole(v, "cache values", k.dtype, shape)
+        _whole(k, "cache keys", dtype, shape)
+        _whole(v, "cache values", dtype, shape)
         _whole(table, "the page table", torch.int32, (B, pages))
         _whole(lens, "the lengths", torch.int32, (B,))
         if weight is not None:
             _whole(weight, "the weights", torch.float32, (B, kv, pages * page))
         if B > 65535 or kv > 1024 or pages * page >= 1 << 30 or total >= 1 << 31:
             raise ValueError("a cache of %d sequences, %d key heads, %d tokens a sequence is too large" % (B, kv, pages * page))
-        _here(_CACHE_NAMES, k, v, table, lens, weight)
+        dev, at = core._dev[0], k.get_device()
+        if at != dev or v.get_device() != at or table.get_device() != at or lens.get_device() != at or (weight is not None and weight.get_device() != at):
+            _here(_CACHE_NAMES, k, v, table, lens, weight)   # (says which; or binds the device at the first call)
         pk, pv = k.data_ptr(), v.data_ptr()
         if (pk | pv) & 15:
             raise ValueError("cache keys and values must start on 16 bytes")
-        self.k, self.v, self.table, self.lens, self.weight = k, v, table, lens, weight
+        self.k, self.v, self.table, self.lens, self.weight, self.dtype = k, v, table, lens, weight, dtype
         self.kv_heads, self.hd, self.page, self.batch, self.pages, self.capacity = kv, hd, page, B, pages, pages * page
         self.c = _CacheC(pk, pv, table.data_ptr(), lens.data_ptr(), None if weight is None else weight.data_ptr(), total, code, kv, page, hd, B, pages)
         self.ref = ctypes.byref(self.c)
@@ -111,10 +114,10 @@ class PagedCache:
 
 def _rows(t, name, cache, shape):
     """t with rows that the kernels can read, and its strides: last dimension dense, every row on 16 bytes (copied where it is not)"""
-    if t.dtype != cache.k.dtype or t.shape != shape:
-        raise ValueError("%s must be %s %s like the cache, got %s %s" % (name, cache.k.dtype, list(shape), t.dtype, list(t.shape)))
-    strides, per = t.stride(), 16 // t.element_size()
-    if strides[-1] != 1 or t.data_ptr() & 15 or any([x % per for x in strides[:-1]]):
+    if t.dtype is not cache.dtype or t.shape != shape:
+        raise ValueError("%s must be %s %s like the cache, got %s %s" % (name, cache.dtype, list(shape), t.dtype, list(t.shape)))
+    strides, per = t.stride(), 3 if cache.c.dtype == 0 else 7   # (elements of 16 bytes, less one)
+    if strides[-1] != 1 or t.data_ptr() & 15 or (strides[0] | strides[1] | strides[-2]) & per:
         t = t.clone(memory_format=torch.contiguous_format)
         strides = t.stride()
     return t, strides
@@ -145,19 +148,19 @@ def cache_append(cache, k, v, counts=None, at=None):
         _chk(rc, "ix_cache_append")
 
 
-_ws_bytes = {}   # workspace of ix_cache_attn by sizes
+_attn_ws_bytes = {}   # workspace of ix_cache_attn by sizes
 
 
 def _attention_ws(cache, H, window, sinks, accumulate):
     c = cache.c
     key = (c.dtype, c.kv_heads, c.page, c.hd, c.batch, c.pages, H, window, sinks, accumulate)
-    need = _ws_bytes.get(key)
+    need = _attn_ws_bytes.get(key)
     if need is None:
         n = ctypes.c_size_t(0)
         _chk(_L().ix_workspace_bytes_cache_attn(cache.ref, H, window, sinks, accumulate, ctypes.byref(n)), "ix_workspace_bytes_cache_attn")
-        if len(_ws_bytes) >= 4096:
-            _ws_bytes.clear()
-        need = _ws_bytes[key] = n.value
+        if len(_attn_ws_bytes) >= 4096:
+            _attn_ws_bytes.clear()
+        need = _attn_ws_bytes[key] = n.value
     return need
 
 
@@ -183,7 +186,7 @@ def cache_attention(q, cache, scale=None, window=None, sinks=0, accumulate=False
     if not math.isfinite(scale):
         raise ValueError("scale must be a finite number, got %r" % scale)
     s = _here(("q",), q)
-    out, ws, need = torch.empty(shape, dtype=q.dtype, device=q.device), None, _attention_ws(cache, H, w, sinks, accumulate)
+    out, ws, need = q.new_empty(shape), None, _attention_ws(cache, H, w, sinks, accumulate)
     if need:   # (a buffer per call: calls on other streams and captured graphs share none)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     rc = _L().ix_cache_attn(cache.ref, q.data_ptr(), qb, qh, out.data_ptr(), H, scale, w, sinks, accumulate, None if ws is None else ws.data_ptr(), need, s)
