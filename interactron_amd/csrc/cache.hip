@@ -379,10 +379,10 @@ __global__ __launch_bounds__(kBlock) void cache_join_kernel(AttnArgs p, int D, i
 // select: the tokens that stay
 // ====================================================================================================================================
 // One workgroup of 16 waves per (sequence, key head).  The r-th largest weight of the middle is found digit by digit (four passes of
-// eight bits over keys whose unsigned order is the weights' order).  Every wave has a stretch of tokens of its own, up to 1024 of them in
+// eight bits over keys whose unsigned order is the weights' order).  Every wave has a stretch of tokens of its own, up to 2048 of them in
 // registers for all passes (longer stretches are read again); at the end it counts what stays of it, the counts are summed in wave order,
 // and it writes its kept indexes with ballots: ascending, and of equal weights the lowest indexes.
-constexpr int kSelBlock = 1024, kSelWaves = 16, kSelHeld = 16;
+constexpr int kSelBlock = 1024, kSelWaves = 16, kSelHeld = 32;
 
 __device__ __forceinline__ unsigned weight_key(float w) {
     if (w != w) return 0u;   // a NaN counts less than every number
@@ -503,7 +503,7 @@ __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, 
 // compact: kept rows to the front, in place
 // ====================================================================================================================================
 // Row i takes what row kept[i] >= i held.  A workgroup walks one column slice of K or V (or the weights) of one (sequence, head) in
-// ascending chunks of 256 rows: all rows of a chunk are in registers before the first of them is written, and no later chunk reads a row
+// ascending chunks of a row a thread: all rows of a chunk are in registers before the first of them is written, and no later chunk reads a row
 // that an earlier one has written, because kept[] ascends and is nowhere below its own place.  So the move needs no second copy of the
 // cache, and the next chunk's rows are on their way while this one is stored, its places (kept index, two page look-ups) a chunk before
 // that, the kept indexes themselves another one.
@@ -513,16 +513,14 @@ struct CompactArgs {
     int budget, row_bytes, slices;   // slices of 16 LANES bytes in a row
 };
 
-constexpr int kChunk = kBlock;   // rows
-
 __device__ __forceinline__ int64_t row_at(const Cache& c, int b, int h, int t) {
     const int64_t r = c.page_row(b, h, t);
     return r < 0 ? -1 : r + (t & ((1 << c.shift) - 1));
 }
 
-template <int LANES>   // threads of a row's slice
-__global__ __launch_bounds__(kBlock) void compact_kernel(CompactArgs p) {
-    constexpr int PER = kBlock / LANES;   // rows of one pass; LANES passes a chunk
+template <int LANES, int THREADS>   // threads of a row's slice, of the workgroup
+__global__ __launch_bounds__(THREADS) void compact_kernel(CompactArgs p) {
+    constexpr int PER = THREADS / LANES, kChunk = THREADS;   // rows of one pass; LANES passes a chunk
     __shared__ int64_t place[4][kChunk][2];
     const int b = blockIdx.z, h = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, cap = p.c.cap();
     const int n = min(max(p.left[b], 0), min(p.budget, cap));
@@ -532,12 +530,12 @@ __global__ __launch_bounds__(kBlock) void compact_kernel(CompactArgs p) {
         if (h == 0 && tid == 0) p.c.lens[b] = n;
         if (!p.c.weight) return;
         float* w = p.c.weight + ((int64_t)b * p.c.kv + h) * cap;
-        for (int i0 = 0; i0 < n; i0 += kBlock * 8) {
+        for (int i0 = 0; i0 < n; i0 += THREADS * 8) {
             float x[8];
             bool move[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const int i = i0 + u * kBlock + tid, from = kept_at(i);
+                const int i = i0 + u * THREADS + tid, from = kept_at(i);
                 move[u] = from > i && from < cap;
                 x[u] = move[u] ? w[from] : 0.f;
             }
@@ -545,7 +543,7 @@ __global__ __launch_bounds__(kBlock) void compact_kernel(CompactArgs p) {
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-                if (move[u]) w[i0 + u * kBlock + tid] = x[u];
+                if (move[u]) w[i0 + u * THREADS + tid] = x[u];
         }
         return;
     }
@@ -780,12 +778,13 @@ extern "C" int ix_cache_compact(const struct ix_paged_cache* cache, const int* k
     p.left = left;
     p.budget = budget;
     p.row_bytes = cache->hd * (cache->dtype == 0 ? 4 : 2);
-    // slices of 128 bytes (a cache line); of 64 where a row has no more, or where that leaves compute units without a workgroup
+    // slices of 128 bytes (a cache line); of 64 where a row has no more, or where that leaves compute units without a workgroup (then with
+    // four times the rows a step: what is left is a chain of steps)
     const bool narrow = p.row_bytes < 128 || (int64_t)cache->batch * cache->kv_heads * 2 * (p.row_bytes / 128) < 256;
     p.slices = p.row_bytes / (narrow ? 64 : 128);
     const dim3 grid(2 * p.slices + 1, cache->kv_heads, cache->batch);
-    if (narrow) compact_kernel<4><<<grid, kBlock, 0, stream>>>(p);
-    else compact_kernel<8><<<grid, kBlock, 0, stream>>>(p);
+    if (narrow) compact_kernel<4, 1024><<<grid, 1024, 0, stream>>>(p);
+    else compact_kernel<8, 256><<<grid, 256, 0, stream>>>(p);
     IX_CHECK_LAUNCH("ix_cache_compact");
     return IX_OK;
 }
