@@ -49,44 +49,116 @@ template <int DT, int D> struct Img {
         }
         return f;
     }
-    // columns d = 16 db + n of rows row0 + 4 g + i and row0 + 16 + 4 g + i (row0 a multiple of 32), for DN values of db from db0 on.
-    // The transposing reads stand in one block with their wait: the compiler would let each of them wait for every request into LDS that
-    // is still on its way, those of the next tiles too.
-    template <int DN> __device__ static __forceinline__ void col_frags(Frag<DT> (&f)[DN], const unsigned char* img, int row0, int db0, int n, int g) {
-        if constexpr (DT == 0) {
+    // Columns d = 16 db + n of rows row0 + 4 g + i and row0 + 16 + 4 g + i (row0 a multiple of 32).  The transposing reads stand in one block
+    // with their wait: the compiler would let each of them wait for every request into LDS that is still on its way, those of the next tiles
+    // too.  Four or eight fragments a block.
+    __device__ static __forceinline__ unsigned col_at(const unsigned char* img, int row0, int db, int n, int g) {
+        const int row = row0 + 4 * g + (n >> 2);
+        return (unsigned)(uintptr_t)(const unsigned char __attribute__((address_space(3)))*)img + row * ROW + ((n & 3) << 3) + ((db ^ turn(row)) << 5);
+    }
+    __device__ static __forceinline__ Frag<DT> col_frag32(const unsigned char* img, int row0, int db, int n, int g) {   // (f32: plain reads)
+        Frag<DT> f;
 #pragma unroll
-            for (int db = 0; db < DN; ++db)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int row = row0 + 16 * (i / 4) + 4 * g + i % 4;
-                    f[db].w[i] = *reinterpret_cast<const unsigned*>(img + row * ROW + (((2 * (db0 + db) + (n >> 3)) ^ turn(row)) << 5) + ((n & 7) << 2));
-                }
-        } else {
-            const int row = row0 + 4 * g + (n >> 2), t = turn(row);
-            const unsigned at = (unsigned)(uintptr_t)(const unsigned char __attribute__((address_space(3)))*)img + row * ROW + ((n & 3) << 3);
-            u32x2 x[DN][2];
-            static_assert(DN == 2 || DN == 4, "");
-#ifdef __HIP_DEVICE_COMPILE__   // (the host's pass does not know the registers' constraint)
-            if constexpr (DN == 2) {
-                asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
-                             "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
-                             : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1])
-                             : "v"(at + ((db0 ^ t) << 5)), "v"(at + (((db0 + 1) ^ t) << 5)), "n"(16 * ROW) : "memory");
-            } else {
-                asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
-                             "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
-                             "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
-                             "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
-                             : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[2][0]), "=&v"(x[2][1]), "=&v"(x[3][0]), "=&v"(x[3][1])
-                             : "v"(at + ((db0 ^ t) << 5)), "v"(at + (((db0 + 1) ^ t) << 5)), "v"(at + (((db0 + 2) ^ t) << 5)), "v"(at + (((db0 + 3) ^ t) << 5)),
-                               "n"(16 * ROW) : "memory");
-            }
-#endif
-#pragma unroll
-            for (int db = 0; db < DN; ++db) { f[db].w[0] = x[db][0].x; f[db].w[1] = x[db][0].y; f[db].w[2] = x[db][1].x; f[db].w[3] = x[db][1].y; }
+        for (int i = 0; i < 8; ++i) {
+            const int row = row0 + 16 * (i / 4) + 4 * g + i % 4;
+            f.w[i] = *reinterpret_cast<const unsigned*>(img + row * ROW + (((2 * db + (n >> 3)) ^ turn(row)) << 5) + ((n & 7) << 2));
         }
+        return f;
     }
 };
+#ifdef __HIP_DEVICE_COMPILE__   // (the host's pass does not know the registers' constraint)
+#define TR_READ(O, A, OFF) "ds_read_b64_tr_b16 %" #O ", %" #A " offset:%" #OFF "\n\t"
+// x[2 i], x[2 i + 1]: rows 4 g .. and 16 + 4 g .. of the column at address i
+template <int HALF> __device__ __forceinline__ void tr_8(u32x2 (&x)[16], const unsigned (&a)[8]) {
+    asm volatile(TR_READ(0, 16, 24) TR_READ(1, 16, 25) TR_READ(2, 17, 24) TR_READ(3, 17, 25) TR_READ(4, 18, 24) TR_READ(5, 18, 25) TR_READ(6, 19, 24)
+                 TR_READ(7, 19, 25) TR_READ(8, 20, 24) TR_READ(9, 20, 25) TR_READ(10, 21, 24) TR_READ(11, 21, 25) TR_READ(12, 22, 24) TR_READ(13, 22, 25)
+                 TR_READ(14, 23, 24) TR_READ(15, 23, 25) "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7]), "=&v"(x[8]), "=&v"(x[9]),
+                   "=&v"(x[10]), "=&v"(x[11]), "=&v"(x[12]), "=&v"(x[13]), "=&v"(x[14]), "=&v"(x[15])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "n"(0), "n"(HALF) : "memory");
+}
+// the same of four addresses, and (x[8 + ..]) of the places 2 HALF behind them
+template <int HALF> __device__ __forceinline__ void tr_4_twice(u32x2 (&x)[16], const unsigned (&a)[4]) {
+    asm volatile(TR_READ(0, 16, 20) TR_READ(1, 16, 21) TR_READ(2, 17, 20) TR_READ(3, 17, 21) TR_READ(4, 18, 20) TR_READ(5, 18, 21) TR_READ(6, 19, 20)
+                 TR_READ(7, 19, 21) TR_READ(8, 16, 22) TR_READ(9, 16, 23) TR_READ(10, 17, 22) TR_READ(11, 17, 23) TR_READ(12, 18, 22) TR_READ(13, 18, 23)
+                 TR_READ(14, 19, 22) TR_READ(15, 19, 23) "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7]), "=&v"(x[8]), "=&v"(x[9]),
+                   "=&v"(x[10]), "=&v"(x[11]), "=&v"(x[12]), "=&v"(x[13]), "=&v"(x[14]), "=&v"(x[15])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(0), "n"(HALF), "n"(2 * HALF), "n"(3 * HALF) : "memory");
+}
+template <int HALF> __device__ __forceinline__ void tr_4(u32x2 (&x)[8], const unsigned (&a)[4]) {
+    asm volatile(TR_READ(0, 8, 12) TR_READ(1, 8, 13) TR_READ(2, 9, 12) TR_READ(3, 9, 13) TR_READ(4, 10, 12) TR_READ(5, 10, 13) TR_READ(6, 11, 12)
+                 TR_READ(7, 11, 13) "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(0), "n"(HALF) : "memory");
+}
+#undef TR_READ
+#else
+template <int HALF> __device__ void tr_8(u32x2 (&x)[16], const unsigned (&a)[8]);
+template <int HALF> __device__ void tr_4_twice(u32x2 (&x)[16], const unsigned (&a)[4]);
+template <int HALF> __device__ void tr_4(u32x2 (&x)[8], const unsigned (&a)[4]);
+#endif
+template <int DT> __device__ __forceinline__ Frag<DT> frag_of(const u32x2& a, const u32x2& b) {
+    Frag<DT> f;
+    f.w[0] = a.x; f.w[1] = a.y; f.w[2] = b.x; f.w[3] = b.y;
+    return f;
+}
+// f[i]: column block db0 + i of image A (rows row0 ..), f[4 + i]: of image B, DN <= 4 of each
+template <int DT, int D, int DN>
+__device__ __forceinline__ void two_images(Frag<DT> (&f)[2][DN], const unsigned char* A, const unsigned char* B, int row0, int db0, int n, int g) {
+    typedef Img<DT, D> I;
+    if constexpr (DT == 0) {
+#pragma unroll
+        for (int i = 0; i < DN; ++i) { f[0][i] = I::col_frag32(A, row0, db0 + i, n, g); f[1][i] = I::col_frag32(B, row0, db0 + i, n, g); }
+    } else if constexpr (DN == 4) {
+        u32x2 x[16];
+        const unsigned a[8] = {I::col_at(A, row0, db0, n, g), I::col_at(A, row0, db0 + 1, n, g), I::col_at(A, row0, db0 + 2, n, g), I::col_at(A, row0, db0 + 3, n, g),
+                               I::col_at(B, row0, db0, n, g), I::col_at(B, row0, db0 + 1, n, g), I::col_at(B, row0, db0 + 2, n, g), I::col_at(B, row0, db0 + 3, n, g)};
+        tr_8<16 * I::ROW>(x, a);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[0][i] = frag_of<DT>(x[2 * i], x[2 * i + 1]); f[1][i] = frag_of<DT>(x[8 + 2 * i], x[8 + 2 * i + 1]); }
+    } else {
+        u32x2 x[8];
+        const unsigned a[4] = {I::col_at(A, row0, db0, n, g), I::col_at(A, row0, db0 + 1, n, g), I::col_at(B, row0, db0, n, g), I::col_at(B, row0, db0 + 1, n, g)};
+        tr_4<16 * I::ROW>(x, a);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { f[0][i] = frag_of<DT>(x[2 * i], x[2 * i + 1]); f[1][i] = frag_of<DT>(x[4 + 2 * i], x[4 + 2 * i + 1]); }
+    }
+}
+// f[kk][i]: column block db0 + i of rows row0 + 32 kk ..
+template <int DT, int D, int KK, int DN>
+__device__ __forceinline__ void one_image(Frag<DT> (&f)[KK][DN], const unsigned char* A, int row0, int db0, int n, int g) {
+    typedef Img<DT, D> I;
+    if constexpr (DT == 0) {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int i = 0; i < DN; ++i) f[kk][i] = I::col_frag32(A, row0 + 32 * kk, db0 + i, n, g);
+    } else if constexpr (DN == 4 && KK == 2) {
+        u32x2 x[16];
+        unsigned a[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = I::col_at(A, row0, db0 + i, n, g);
+        tr_4_twice<16 * I::ROW>(x, a);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[0][i] = frag_of<DT>(x[2 * i], x[2 * i + 1]); f[1][i] = frag_of<DT>(x[8 + 2 * i], x[8 + 2 * i + 1]); }
+    } else if constexpr (DN == 4) {
+        u32x2 x[8];
+        const unsigned a[4] = {I::col_at(A, row0, db0, n, g), I::col_at(A, row0, db0 + 1, n, g), I::col_at(A, row0, db0 + 2, n, g), I::col_at(A, row0, db0 + 3, n, g)};
+        tr_4<16 * I::ROW>(x, a);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[0][i] = frag_of<DT>(x[2 * i], x[2 * i + 1]);
+    } else {   // head dim 32: two column blocks
+        static_assert(DN == 2 && KK <= 2, "");
+        u32x2 x[8];
+        const unsigned a[4] = {I::col_at(A, row0, 0, n, g), I::col_at(A, row0, 1, n, g), I::col_at(A, row0 + 32 * (KK - 1), 0, n, g), I::col_at(A, row0 + 32 * (KK - 1), 1, n, g)};
+        tr_4<16 * I::ROW>(x, a);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) f[kk][i] = frag_of<DT>(x[4 * kk + 2 * i], x[4 * kk + 2 * i + 1]);
+    }
+}
 static_assert(Img<1, 128>::PAIRS == 8 && Img<1, 32>::SWEEP == 4, "image geometry");
 
 // A tile of ROWS rows from memory to LDS without registers: every lane names the 16 bytes that belong at its place of the image
@@ -371,19 +443,25 @@ __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) 
                             sum[nb] += s[nb][sb][r];
                         }
                 }
+                // 32-row steps whose columns come in one block of reads (head dim 128: four column blocks of one step; more at once was no faster)
+                constexpr int KK = SB / 2, TOGETHER = I::DB == 8 ? 1 : KK;
 #pragma unroll
-                for (int kk = 0; kk < SB / 2; ++kk) {
-                    Frag<DT> pf[NB];
+                for (int k0 = 0; k0 < KK; k0 += TOGETHER) {
+                    Frag<DT> pf[TOGETHER][NB];
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) pf[nb] = as_frag<DT>(s[nb][2 * kk], s[nb][2 * kk + 1]);
+                    for (int kk = 0; kk < TOGETHER; ++kk)
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) pf[kk][nb] = as_frag<DT>(s[nb][2 * (k0 + kk)], s[nb][2 * (k0 + kk) + 1]);
 #pragma unroll
                     for (int d0 = 0; d0 < I::DB; d0 += I::DN) {
-                        Frag<DT> vf[I::DN];
-                        I::col_frags(vf, vi, 32 * kk, d0, n16, g);
+                        Frag<DT> vf[TOGETHER][I::DN];
+                        one_image<DT, D>(vf, vi, 32 * k0, d0, n16, g);
 #pragma unroll
-                        for (int db = 0; db < I::DN; ++db)
+                        for (int kk = 0; kk < TOGETHER; ++kk)
 #pragma unroll
-                            for (int nb = 0; nb < NB; ++nb) o[nb][d0 + db] = seq_mma<DT>(vf[db], pf[nb], o[nb][d0 + db]);
+                            for (int db = 0; db < I::DN; ++db)
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb) o[nb][d0 + db] = seq_mma<DT>(vf[kk][db], pf[kk][nb], o[nb][d0 + db]);
                     }
                 }
             }
@@ -591,14 +669,14 @@ __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, i
                     }
 #pragma unroll
                     for (int d0 = 0; d0 < I::DB; d0 += I::DN) {
-                        Frag<DT> kf[I::DN];
-                        I::col_frags(kf, ki, 32 * kk, d0, n16, g);
+                        Frag<DT> kc[1][I::DN];
+                        one_image<DT, D>(kc, ki, 32 * kk, d0, n16, g);
 #pragma unroll
                         for (int db = 0; db < I::DN; ++db)
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
-                                if constexpr (DT != 0) acc[nb][d0 + db] = seq_mma<DT>(kf[db], zr[nb], acc[nb][d0 + db]);
-                                acc[nb][d0 + db] = seq_mma<DT>(kf[db], zf[nb], acc[nb][d0 + db]);
+                                if constexpr (DT != 0) acc[nb][d0 + db] = seq_mma<DT>(kc[0][db], zr[nb], acc[nb][d0 + db]);
+                                acc[nb][d0 + db] = seq_mma<DT>(kc[0][db], zf[nb], acc[nb][d0 + db]);
                             }
                     }
                 }
@@ -756,16 +834,15 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
                     }
 #pragma unroll
                     for (int d0 = 0; d0 < I::DB; d0 += I::DN) {
-                        Frag<DT> gf[I::DN], qf[I::DN];
-                        I::col_frags(gf, gi, 32 * kk, d0, n16, g);
-                        I::col_frags(qf, qi, 32 * kk, d0, n16, g);
+                        Frag<DT> gq[2][I::DN];   // columns of do, of q
+                        two_images<DT, D, I::DN>(gq, gi, qi, 32 * kk, d0, n16, g);
 #pragma unroll
                         for (int db = 0; db < I::DN; ++db)
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
-                                av[nb][d0 + db] = seq_mma<DT>(gf[db], pf[nb], av[nb][d0 + db]);
-                                if constexpr (DT != 0) ak[nb][d0 + db] = seq_mma<DT>(qf[db], zr[nb], ak[nb][d0 + db]);
-                                ak[nb][d0 + db] = seq_mma<DT>(qf[db], zf[nb], ak[nb][d0 + db]);
+                                av[nb][d0 + db] = seq_mma<DT>(gq[0][db], pf[nb], av[nb][d0 + db]);
+                                if constexpr (DT != 0) ak[nb][d0 + db] = seq_mma<DT>(gq[1][db], zr[nb], ak[nb][d0 + db]);
+                                ak[nb][d0 + db] = seq_mma<DT>(gq[1][db], zf[nb], ak[nb][d0 + db]);
                             }
                     }
                 }
@@ -886,7 +963,9 @@ KeyPlan key_plan(const ix_band* s) {
     r.splits = (int)(sp < 1 ? 1 : sp);
     const int64_t piece = div_up(each, r.splits);
     int64_t ws = 2 * all * group <= 5 * piece ? 1 : div_up(all * group, 2 * piece);
-    if (r.splits > 1 && ws < r.splits) ws = r.splits;
+    const int64_t wide = (int64_t)s->batch * s->kv_heads * r.wide;
+    if (wide && ws > div_up(1024, wide)) ws = div_up(1024, wide);   // (many such blocks fill the compute units by themselves)
+    if (ws < r.splits) ws = r.splits;
     r.wide_splits = (int)(ws > 64 ? 64 : ws);
     r.items = r.wide * r.wide_splits + (r.blocks - r.wide) * r.splits;
     return r;
@@ -903,7 +982,7 @@ int band_of(BandArgs& a, const ix_band* s, const char* who) {
     IX_CHECK_ARG(s, "%s: null description", who);
     IX_CHECK_ARG(s->dtype >= 0 && s->dtype <= 2, "%s: dtype %d is none of 0 (f32), 1 (bf16), 2 (fp16)", who, s->dtype);
     IX_CHECK_ARG(s->hd == 32 || s->hd == 64 || s->hd == 128, "%s: head dim %d is none of 32, 64, 128", who, s->hd);
-    IX_CHECK_ARG(s->batch > 0 && s->Lq > 0 && s->Lk > 0 && s->Lq < (1 << 22) && s->Lk < (1 << 22), "%s: bad sizes (batch %d, %d queries, %d keys)", who,
+    IX_CHECK_ARG(s->batch > 0 && s->Lq > 0 && s->Lk > 0 && s->Lq <= 65535 * 64 && s->Lk <= 65535 * 64, "%s: bad sizes (batch %d, %d queries, %d keys)", who,
                  s->batch, s->Lq, s->Lk);
     IX_CHECK_ARG(s->heads > 0 && s->kv_heads > 0 && s->heads % s->kv_heads == 0, "%s: %d query heads over %d key heads", who, s->heads, s->kv_heads);
     IX_CHECK_ARG((int64_t)s->batch * s->heads < (1 << 30), "%s: too many heads", who);

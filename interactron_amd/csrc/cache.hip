@@ -674,6 +674,8 @@ extern "C" int ix_cache_append(const struct ix_paged_cache* cache, const void* k
     IX_CHECK_ARG(T >= 0 && T < (1 << 30), "ix_cache_append: T=%d", T);
     IX_CHECK_ARG(T == 0 || (k && v && ix_al16(k) && ix_al16(v)), "ix_cache_append: null or unaligned rows");
     for (int64_t s : {sb_k, st_k, sh_k, sb_v, st_v, sh_v}) IX_CHECK_ARG(s * eb % 16 == 0, "ix_cache_append: rows that do not start on 16 bytes");
+    for (const int* x : {counts, at})   // (the lengths themselves may be named; another part of their memory would change under the call)
+        IX_CHECK_ARG(!x || x == c.lens || x + c.batch <= c.lens || c.lens + c.batch <= x, "ix_cache_append: counts or at overlap the lengths");
     AppendArgs p{c, static_cast<const unsigned char*>(k), static_cast<const unsigned char*>(v), sb_k * eb, st_k * eb, sh_k * eb, sb_v * eb, st_v * eb,
                  sh_v * eb, counts, at, T, cache->hd * eb / 16, 0, 0};
     // a workgroup moves up to 1 024 16-byte chunks of K and as many of V: four of each per thread
@@ -763,7 +765,7 @@ extern "C" int ix_cache_select(const float* weight, const int* lens, int* kept, 
     IX_CHECK_ARG(budget > 0 && sinks >= 0 && recent >= 0 && (int64_t)sinks + recent <= budget, "ix_cache_select: %d first and %d last tokens do not fit into %d",
                  sinks, recent, budget);
     IX_CHECK_ARG(budget <= capacity, "ix_cache_select: a budget of %d for a capacity of %d", budget, capacity);
-    IX_CHECK_ARG(left != lens, "ix_cache_select: the lengths are still read while the new ones are written");
+    IX_CHECK_ARG(left + batch <= lens || lens + batch <= left, "ix_cache_select: the lengths are still read while the new ones are written");
     select_kernel<<<dim3(kv_heads, batch), kSelBlock, 0, stream>>>(weight, lens, kept, left, kv_heads, capacity, budget, sinks, recent);
     IX_CHECK_LAUNCH("ix_cache_select");
     return IX_OK;
@@ -773,7 +775,7 @@ extern "C" int ix_cache_compact(const struct ix_paged_cache* cache, const int* k
     CompactArgs p;
     if (int rc = cache_of(p.c, cache, "ix_cache_compact")) return rc;
     IX_CHECK_ARG(kept && left && budget > 0, "ix_cache_compact: null pointer or empty budget");
-    IX_CHECK_ARG(left != cache->lens, "ix_cache_compact: the new lengths are the cache's own");
+    IX_CHECK_ARG(left + cache->batch <= cache->lens || cache->lens + cache->batch <= left, "ix_cache_compact: the new lengths overlap the cache's own");
     p.kept = kept;
     p.left = left;
     p.budget = budget;

@@ -22,6 +22,7 @@ class _BandC(ctypes.Structure):   # struct ix_band of include/interactron_hip.h
 
 
 _NAMES = ("q", "k", "v", "q_lens", "kv_lens")
+_LONGEST = 65535 * 64   # rows: blocks of 64 along one axis of a launch
 
 
 def _dense_rows(t):
@@ -123,7 +124,7 @@ def band_attention(q, k, v, window=None, sinks=0, causal=True, scale=None, q_len
         raise ValueError("a head dim of %d: %s are supported" % (D, _HEAD_DIMS))
     if k.shape[2] == 0 or H == 0 or H % k.shape[2]:
         raise ValueError("%d query heads over %d key heads" % (H, k.shape[2]))
-    if max(Lq, k.shape[1]) >= 1 << 22 or B * H >= 1 << 30:
+    if max(Lq, k.shape[1]) > _LONGEST or B * H >= 1 << 30:
         raise ValueError("%d queries and %d keys of %d heads are too many" % (Lq, k.shape[1], B * H))
     for t, name in ((q_lens, "q_lens"), (kv_lens, "kv_lens")):
         if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):

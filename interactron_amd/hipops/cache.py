@@ -76,8 +76,15 @@ class PagedCache:
              sequences may share pages that both only read.
     lens     int32 [batch]: tokens held
     weight   float32 [batch, kv_heads, pages * page] or None: the attention each token has had so far
+    The tensors are written in place and cannot be exchanged for others (make another cache: it costs nothing but the checks).
     """
-    __slots__ = ("k", "v", "table", "lens", "weight", "kv_heads", "hd", "page", "batch", "pages", "capacity", "dtype", "c", "ref")
+    __slots__ = ("_k", "_v", "_table", "_lens", "_weight", "kv_heads", "hd", "page", "batch", "pages", "capacity", "dtype", "c", "ref")
+
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    table = property(lambda self: self._table)
+    lens = property(lambda self: self._lens)
+    weight = property(lambda self: self._weight)
 
     def __init__(self, k, v, table, lens, weight=None):
         shape, dtype = k.shape, k.dtype
@@ -106,7 +113,7 @@ class PagedCache:
         pk, pv = k.data_ptr(), v.data_ptr()
         if (pk | pv) & 15:
             raise ValueError("cache keys and values must start on 16 bytes")
-        self.k, self.v, self.table, self.lens, self.weight, self.dtype = k, v, table, lens, weight, dtype
+        self._k, self._v, self._table, self._lens, self._weight, self.dtype = k, v, table, lens, weight, dtype
         self.kv_heads, self.hd, self.page, self.batch, self.pages, self.capacity = kv, hd, page, B, pages, pages * page
         self.c = _CacheC(pk, pv, table.data_ptr(), lens.data_ptr(), None if weight is None else weight.data_ptr(), total, code, kv, page, hd, B, pages)
         self.ref = ctypes.byref(self.c)
@@ -134,7 +141,7 @@ def cache_append(cache, k, v, counts=None, at=None):
 
     at: int32 [B], default: the cache's lengths (the new tokens follow the old ones; an earlier place takes tokens back).  counts: int32
     [B], default T (rows behind a sequence's count are padding and not read).  Tokens beyond the capacity are dropped.  New tokens have
-    had no attention yet: their weight is 0."""
+    had no attention yet: their weight is 0.  k and v must not be parts of the cache's own pools."""
     if k.dim() != 4:
         raise ValueError("new keys must be [batch, tokens, kv_heads, hd], got %s" % list(k.shape))
     T = k.shape[1]
@@ -142,6 +149,8 @@ def cache_append(cache, k, v, counts=None, at=None):
     k, (kb, kt, kh, _) = _rows(k, "new keys", cache, shape)
     v, (vb, vt, vh, _) = _rows(v, "new values", cache, shape)
     n, start = _per_sequence(counts, "counts", cache), _per_sequence(at, "at", cache)
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        raise _lib.HipLibraryError("cache_append has no backward: call it under torch.no_grad()")
     s = _here(("new keys", "new values", "counts", "at"), k, v, counts, at)
     rc = _L().ix_cache_append(cache.ref, k.data_ptr(), v.data_ptr(), T, kb, kt, kh, vb, vt, vh, n, start, s)
     if rc:
@@ -227,7 +236,7 @@ def cache_compact(cache, kept, left):
     _whole(left, "left", torch.int32, (cache.batch,))
     if kept.shape[2] > cache.capacity:
         raise ValueError("kept names %d tokens, the capacity is %d" % (kept.shape[2], cache.capacity))
-    if left.data_ptr() == cache.lens.data_ptr():
+    if abs(left.data_ptr() - cache.lens.data_ptr()) < 4 * cache.batch:
         raise ValueError("left must not be the cache's own lengths")
     s = _here(("kept", "left"), kept, left)
     _chk(_L().ix_cache_compact(cache.ref, kept.data_ptr(), left.data_ptr(), kept.shape[2], s), "ix_cache_compact")

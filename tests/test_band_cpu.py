@@ -45,7 +45,7 @@ def c_band(**change):
     return hipops.band._BandC(*[f[n] for n, _ in hipops.band._BandC._fields_])
 
 
-@pytest.mark.parametrize("change", [dict(q=None), dict(k=None), dict(v=4100), dict(dtype=3), dict(hd=80), dict(batch=0), dict(Lq=0), dict(Lk=0), dict(Lq=1 << 22),
+@pytest.mark.parametrize("change", [dict(q=None), dict(k=None), dict(v=4100), dict(dtype=3), dict(hd=80), dict(batch=0), dict(Lq=0), dict(Lk=0), dict(Lq=65535 * 64 + 1), dict(Lk=65535 * 64 + 1),
                                     dict(heads=3), dict(kv_heads=0), dict(heads=0), dict(window=-1), dict(sinks=-1), dict(scale=float("nan")),
                                     dict(scale=float("inf")), dict(q_sl=252), dict(v_sh=33), dict(batch=1 << 29)], ids=str)
 def test_c_entries_refuse_a_bad_description(change):

@@ -90,18 +90,19 @@ def test_c_entries_refuse_a_bad_cache(change):
     ("append", dict(T=-1), -1), ("append", dict(k=None), -1), ("append", dict(v=4104), -1), ("append", dict(st=60), -1),
     ("compact", dict(kept=None), -1), ("compact", dict(left=None), -1), ("compact", dict(left=8192), -1), ("compact", dict(budget=0), -1),
     ("select", dict(weight=None), -1), ("select", dict(budget=0), -1), ("select", dict(budget=64), -1), ("select", dict(sinks=5, recent=4), -1),
-    ("select", dict(sinks=-1), -1), ("select", dict(batch=0), -1), ("select", dict(lens=12288), -1),
+    ("select", dict(sinks=-1), -1), ("select", dict(batch=0), -1), ("select", dict(lens=12288), -1), ("select", dict(lens=12292), -1),
+    ("compact", dict(left=8196), -1), ("append", dict(counts=8196), -1), ("append", dict(at=8188), -1),
 ])
 def test_c_entries_refuse_bad_arguments(entry, args, code):
     L = _lib.load()
     a = dict(q=4096, sq_b=256, sq_h=64, out=4096, heads=4, window=0, sinks=0, accumulate=0, ws=None, nbytes=0, k=4096, v=4096, T=1, st=128, kept=4096,
-             left=12288, budget=8, weight=4096, lens=8192, batch=2, recent=0)
+             left=12288, budget=8, weight=4096, lens=8192, batch=2, recent=0, counts=None, at=None)
     a.update(args)
     c = c_cache(lens=8192, weight=a["weight"])
     if entry == "attn":
         rc = L.ix_cache_attn(ctypes.byref(c), a["q"], a["sq_b"], a["sq_h"], a["out"], a["heads"], 0.125, a["window"], a["sinks"], a["accumulate"], a["ws"], a["nbytes"], None)
     elif entry == "append":
-        rc = L.ix_cache_append(ctypes.byref(c), a["k"], a["v"], a["T"], 128, a["st"], 64, 128, 128, 64, None, None, None)
+        rc = L.ix_cache_append(ctypes.byref(c), a["k"], a["v"], a["T"], 128, a["st"], 64, 128, 128, 64, a["counts"], a["at"], None)
     elif entry == "compact":
         rc = L.ix_cache_compact(ctypes.byref(c), a["kept"], a["left"], a["budget"], None)
     else:

@@ -259,6 +259,20 @@ def test_append_refuses():
             hipops.cache_append(cache, k, k, **how)
     with pytest.raises(_lib.HipLibraryError, match="GPU"):
         hipops.cache_append(cache, k, k.cpu())
+    with pytest.raises(_lib.HipLibraryError, match="no backward"):
+        hipops.cache_append(cache, k.clone().requires_grad_(True), k)
+    base = torch.zeros(3, dtype=torch.int32, device="cuda")
+    shared = hipops.PagedCache(cache.k, cache.v, cache.table, base[:2])
+    for how in (dict(at=base[1:]), dict(counts=base[1:])):
+        with pytest.raises(_lib.HipLibraryError, match="overlap"):
+            hipops.cache_append(shared, k, k, **how)
+
+
+def test_the_cache_keeps_its_tensors():
+    cache = make([4, 4])
+    for name in ("k", "v", "table", "lens", "weight"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name).clone())
 
 
 # ---- select and compact -------------------------------------------------------------------------------------------------------------
