@@ -537,7 +537,8 @@ int ix_adam_step_f32(float* p, float* g, float* m, float* v, int64_t n, float lr
  * all) or j < sinks; with `causal` also j <= p.  q [batch][Lq][heads][hd], k, v [batch][Lk][kv_heads][hd] by element strides (sb, sl,
  * sh; rows dense and on 16 bytes); query head h reads key head h / (heads / kv_heads).  dtype 0 f32, 1 bf16, 2 fp16; hd 32, 64, 128.
  * q_lens, kv_lens int32 [batch] (null: Lq, Lk): rows behind them are never read and come back as zeros.  A query that sees nothing
- * gives zeros and has no gradient.  Keys and values that a query does not see have to be finite where they lie inside the lengths.
+ * gives zeros and has no gradient.  Inside the lengths v has to be finite also where a query does not see it, for the gradients q, k
+ * and d_out too.  batch * heads < 2^24.
  *   ix_band_attn_fwd : out [batch][Lq][heads][hd] dense; for the gradients (may be null) lse f32 [batch][heads][pitch], base 2 (pitch
  *                      from ix_band_attn_lse_pitch), and rest like out: what its rounding to 16 bits took away (not with f32).  Few
  *                      rows over many keys go in pieces that are joined: workspace of ix_workspace_bytes_band_attn_fwd bytes (often 0)

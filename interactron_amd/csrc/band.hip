@@ -19,8 +19,9 @@ namespace {
 
 constexpr int kBlock = 256, kWaves = 4;
 constexpr int kFar = 1 << 30;   // an unlimited band (lengths stay below 2^28)
+constexpr int64_t kMostGroups = 1 << 24;   // workgroups along x: a launch counts its threads in 32 bits
 
-// owner rows of a wave: two blocks of 16 with 16-bit operands, one with f32 (twice the registers an element)
+// owner rows of a workgroup: one or two blocks of 16 a wave
 constexpr int owner_rows(int nb) { return 16 * nb * kWaves; }
 constexpr int key_tile(int dt) { return dt == 0 ? 32 : 64; }
 constexpr int query_tile(int dt, int hd) { return dt == 0 || hd == 128 ? 32 : 64; }
@@ -985,7 +986,7 @@ int band_of(BandArgs& a, const ix_band* s, const char* who) {
     IX_CHECK_ARG(s->batch > 0 && s->Lq > 0 && s->Lk > 0 && s->Lq <= 65535 * 64 && s->Lk <= 65535 * 64, "%s: bad sizes (batch %d, %d queries, %d keys)", who,
                  s->batch, s->Lq, s->Lk);
     IX_CHECK_ARG(s->heads > 0 && s->kv_heads > 0 && s->heads % s->kv_heads == 0, "%s: %d query heads over %d key heads", who, s->heads, s->kv_heads);
-    IX_CHECK_ARG((int64_t)s->batch * s->heads < (1 << 30), "%s: too many heads", who);
+    IX_CHECK_ARG((int64_t)s->batch * s->heads < kMostGroups, "%s: too many heads", who);
     IX_CHECK_ARG(s->window >= 0 && s->sinks >= 0, "%s: negative window or sinks", who);
     IX_CHECK_ARG(s->scale == s->scale && s->scale < INFINITY && s->scale > -INFINITY, "%s: the scale is no number", who);
     IX_CHECK_ARG(s->q && s->k && s->v && ix_al16(s->q) && ix_al16(s->k) && ix_al16(s->v), "%s: null or unaligned q, k or v", who);
@@ -1117,7 +1118,7 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
     const int nb = bwd_nb(s), rows = owner_rows(nb);
     const int64_t key_groups = (int64_t)a.B * a.kv * r.items, groups = key_groups + (int64_t)a.B * a.H * ((a.Lq + rows - 1) / rows);
     const int64_t delta_groups = ((int64_t)a.B * a.H * a.Lp * (s->hd * eb / 16) + kBlock - 1) / kBlock;
-    IX_CHECK_ARG(groups < (1ll << 31) && delta_groups < (1ll << 31), "ix_band_attn_bwd: too many rows for one launch");
+    IX_CHECK_ARG(groups < kMostGroups && delta_groups < kMostGroups, "ix_band_attn_bwd: too many rows for one launch");
     a.key_groups = (int)key_groups;
 #define BAND_DELTA(DT, D) band_delta_kernel<DT, D><<<(unsigned)delta_groups, kBlock, 0, stream>>>(a)
     BAND_GO(BAND_DELTA)

@@ -11,6 +11,7 @@
 namespace {
 
 constexpr int kBlock = 256;
+constexpr int64_t kMostGroups = 1 << 24;   // workgroups along x: a launch counts its threads in 32 bits
 
 struct Cache {   // (the launch argument form of ix_paged_cache)
     unsigned char *k, *v;
@@ -684,7 +685,7 @@ extern "C" int ix_cache_append(const struct ix_paged_cache* cache, const void* k
     const bool one = items <= p.per_block;
     int64_t blocks = (items + p.per_block - 1) / p.per_block;
     if (blocks < 1) blocks = 1;
-    IX_CHECK_ARG(blocks < (1ll << 31), "ix_cache_append: too many rows");
+    IX_CHECK_ARG(blocks < kMostGroups, "ix_cache_append: too many rows");
     // (lengths that are read as starts must not change under the other workgroups of the sequence)
     p.set_lens = one || (at && at != c.lens && counts != c.lens);
     append_kernel<<<dim3((unsigned)blocks, c.batch), kBlock, 0, stream>>>(p);
@@ -741,7 +742,7 @@ extern "C" int ix_cache_attn(const struct ix_paged_cache* cache, const void* q, 
     p.accumulate = accumulate != 0;
     const int64_t wblocks = accumulate ? ((int64_t)r.max_tiles * r.kt + 1023) / 1024 : 0, oblocks = (int64_t)cache->batch * heads;
     const int64_t jblocks = oblocks + wblocks * cache->batch * cache->kv_heads;
-    IX_CHECK_ARG((int64_t)cache->kv_heads * r.qtiles <= 65535 && jblocks < (1ll << 31), "ix_cache_attn: too many heads or tokens for one launch");
+    IX_CHECK_ARG((int64_t)cache->kv_heads * r.qtiles <= 65535 && jblocks < kMostGroups, "ix_cache_attn: too many heads or tokens for one launch");
     const dim3 grid(r.splits, cache->kv_heads * r.qtiles, cache->batch);
 #define CACHE_GO(DT, D)                                                                       \
     { if (r.waves == 8) cache_attn_kernel<DT, D, 8><<<grid, 512, 0, stream>>>(p);             \
@@ -761,7 +762,7 @@ extern "C" int ix_cache_attn(const struct ix_paged_cache* cache, const void* q, 
 extern "C" int ix_cache_select(const float* weight, const int* lens, int* kept, int* left, int batch, int kv_heads, int capacity, int budget, int sinks,
                                int recent, hipStream_t stream) {
     IX_CHECK_ARG(weight && lens && kept && left, "ix_cache_select: null pointer");
-    IX_CHECK_ARG(batch > 0 && batch <= 65535 && kv_heads > 0 && capacity > 0 && capacity < (1 << 30), "ix_cache_select: bad sizes");
+    IX_CHECK_ARG(batch > 0 && batch <= 65535 && kv_heads > 0 && kv_heads < (1 << 20) && capacity > 0 && capacity < (1 << 30), "ix_cache_select: bad sizes");
     IX_CHECK_ARG(budget > 0 && sinks >= 0 && recent >= 0 && (int64_t)sinks + recent <= budget, "ix_cache_select: %d first and %d last tokens do not fit into %d",
                  sinks, recent, budget);
     IX_CHECK_ARG(budget <= capacity, "ix_cache_select: a budget of %d for a capacity of %d", budget, capacity);

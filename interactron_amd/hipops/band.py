@@ -113,7 +113,9 @@ def band_attention(q, k, v, window=None, sinks=0, causal=True, scale=None, q_len
     padded batch; padding is never read and comes back as zeros.  A query that sees nothing gives zeros and has no gradient.
 
     float32, bfloat16 or float16 with sums and softmax in 32 bits, hd 32, 64 or 128, rows with any strides (a slice of a packed projection
-    is taken as it is).  Differentiable once.  Values have to be finite inside the lengths, also those a query does not see."""
+    is taken as it is).  Differentiable once.  Inside the lengths, values have to be finite also where a query does not see them, and for the
+    gradients queries, keys and the gradient of the output too: there a weight of zero is multiplied with them.  A captured backward pass
+    has leaves of its own: no eager graph of the same leaves may be alive."""
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         if t.dim() != 4 or t.dtype not in _DTYPES or t.dtype != q.dtype:
             raise ValueError("%s must be [batch, length, heads, hd] in float32, bfloat16 or float16 like q, got %s %s" % (name, t.dtype, list(t.shape)))
@@ -124,7 +126,7 @@ def band_attention(q, k, v, window=None, sinks=0, causal=True, scale=None, q_len
         raise ValueError("a head dim of %d: %s are supported" % (D, _HEAD_DIMS))
     if k.shape[2] == 0 or H == 0 or H % k.shape[2]:
         raise ValueError("%d query heads over %d key heads" % (H, k.shape[2]))
-    if max(Lq, k.shape[1]) > _LONGEST or B * H >= 1 << 30:
+    if max(Lq, k.shape[1]) > _LONGEST or B * H >= 1 << 24:
         raise ValueError("%d queries and %d keys of %d heads are too many" % (Lq, k.shape[1], B * H))
     for t, name in ((q_lens, "q_lens"), (kv_lens, "kv_lens")):
         if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):

@@ -72,11 +72,12 @@ class PagedCache:
 
     k, v     [pages_total, kv_heads, page, hd], float32, bfloat16 or float16; hd 32, 64 or 128; page a power of two, 16 .. 1024
     table    int32 [batch, pages]: the pages of every sequence in order; token t is row t % page of page table[b, t // page].  Entries
-             behind a sequence's length are not read; one that is outside the pool counts as masked and is never written through.  Two
-             sequences may share pages that both only read.
+             behind a sequence's length may hold anything; one that is outside the pool counts as masked and is never written through.
+             Sequences may share pages that all of them only read; a page that is written has one place in the table.
     lens     int32 [batch]: tokens held
     weight   float32 [batch, kv_heads, pages * page] or None: the attention each token has had so far
-    The tensors are written in place and cannot be exchanged for others (make another cache: it costs nothing but the checks).
+    The tensors are written in place, so none of them may require a gradient, and they cannot be exchanged for others (make another cache:
+    it costs nothing but the checks).
     """
     __slots__ = ("_k", "_v", "_table", "_lens", "_weight", "kv_heads", "hd", "page", "batch", "pages", "capacity", "dtype", "c", "ref")
 
@@ -107,6 +108,8 @@ class PagedCache:
             _whole(weight, "the weights", torch.float32, (B, kv, pages * page))
         if B > 65535 or kv > 1024 or pages * page >= 1 << 30 or total >= 1 << 31:
             raise ValueError("a cache of %d sequences, %d key heads, %d tokens a sequence is too large" % (B, kv, pages * page))
+        if k.requires_grad or v.requires_grad or (weight is not None and weight.requires_grad):
+            raise _lib.HipLibraryError("the tensors of a cache are written in place: none of them may require a gradient")
         dev, at = core._dev[0], k.get_device()
         if at != dev or v.get_device() != at or table.get_device() != at or lens.get_device() != at or (weight is not None and weight.get_device() != at):
             _here(_CACHE_NAMES, k, v, table, lens, weight)   # (says which; or binds the device at the first call)
@@ -139,8 +142,8 @@ def _per_sequence(t, name, cache):
 def cache_append(cache, k, v, counts=None, at=None):
     """Writes k, v [B, T, kv_heads, hd] as tokens at[b] .. at[b] + counts[b] - 1 of every sequence and sets the lengths to at + counts.
 
-    at: int32 [B], default: the cache's lengths (the new tokens follow the old ones; an earlier place takes tokens back).  counts: int32
-    [B], default T (rows behind a sequence's count are padding and not read).  Tokens beyond the capacity are dropped.  New tokens have
+    at: int32 [B], default: the cache's lengths (the new tokens follow the old ones; an earlier place takes tokens back, behind a later one
+    lies whatever the pages held).  counts: int32 [B], default T (rows behind a sequence's count are padding and not read).  Tokens beyond the capacity are dropped.  New tokens have
     had no attention yet: their weight is 0.  k and v must not be parts of the cache's own pools."""
     if k.dim() != 4:
         raise ValueError("new keys must be [batch, tokens, kv_heads, hd], got %s" % list(k.shape))

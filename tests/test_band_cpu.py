@@ -30,6 +30,12 @@ def test_wrong_arguments_are_refused(shape, how, words):
         hipops.band_attention(*qkv(**shape), **how)
 
 
+def test_too_many_heads_for_a_launch_are_refused():
+    q, k = torch.zeros(1, 1, 1, 64, dtype=BF16).expand(1 << 22, 1, 4, 64), torch.zeros(1, 1, 1, 64, dtype=BF16).expand(1 << 22, 1, 1, 64)
+    with pytest.raises(ValueError, match="too many"):
+        hipops.band_attention(q, k, k)
+
+
 @pytest.mark.parametrize("change", [lambda q, k, v: (q[0], k, v), lambda q, k, v: (q, k.float(), v), lambda q, k, v: (q, k, v[:, :3]),
                                     lambda q, k, v: (q[:1], k, v), lambda q, k, v: (q[..., :32], k, v), lambda q, k, v: (q, k[:, :, :1], v)])
 def test_tensors_that_do_not_fit_are_refused(change):
@@ -47,7 +53,7 @@ def c_band(**change):
 
 @pytest.mark.parametrize("change", [dict(q=None), dict(k=None), dict(v=4100), dict(dtype=3), dict(hd=80), dict(batch=0), dict(Lq=0), dict(Lk=0), dict(Lq=65535 * 64 + 1), dict(Lk=65535 * 64 + 1),
                                     dict(heads=3), dict(kv_heads=0), dict(heads=0), dict(window=-1), dict(sinks=-1), dict(scale=float("nan")),
-                                    dict(scale=float("inf")), dict(q_sl=252), dict(v_sh=33), dict(batch=1 << 29)], ids=str)
+                                    dict(scale=float("inf")), dict(q_sl=252), dict(v_sh=33), dict(batch=1 << 29), dict(batch=1 << 22)], ids=str)
 def test_c_entries_refuse_a_bad_description(change):
     L, c, n = _lib.load(), c_band(**change), ctypes.c_size_t(0)
     for rc in (L.ix_band_attn_fwd(ctypes.byref(c), 4096, 4096, 4096, 4096, 1 << 30, None), L.ix_workspace_bytes_band_attn_fwd(ctypes.byref(c), ctypes.byref(n)), L.ix_workspace_bytes_band_attn_bwd(ctypes.byref(c), ctypes.byref(n)),
@@ -72,3 +78,9 @@ def test_c_entries_refuse_bad_buffers():
         assert L.ix_band_attn_fwd(ctypes.byref(few), 4096, None, None, ws, size, None) == -3
     p = ctypes.c_int64(0)
     assert L.ix_band_attn_lse_pitch(0, ctypes.byref(p)) == -1 and L.ix_band_attn_lse_pitch(129, ctypes.byref(p)) == 0 and p.value == 256
+
+
+def test_c_gradients_refuse_more_rows_than_a_launch_has():
+    L, c = _lib.load(), c_band(batch=1 << 12, Lq=65535 * 64)
+    assert L.ix_band_attn_bwd(ctypes.byref(c), 4096, 4096, 4096, 4096, 1280, 256, 64, 4096, 4096, 4096, 4096, 1 << 62, None) == -1
+    assert b"too many rows" in L.ix_last_error()

@@ -42,6 +42,14 @@ def test_cache_of_the_wrong_form_is_refused(change, words):
         hipops.PagedCache(**dict(parts(), **change))
 
 
+@pytest.mark.parametrize("name", ["k", "v", "weight"])
+def test_cache_tensors_with_a_gradient_are_refused(name):
+    made = dict(parts(), weight=torch.zeros(2, 2, 48))
+    made[name].requires_grad_(True)
+    with pytest.raises(_lib.HipLibraryError, match="gradient"):
+        hipops.PagedCache(**made)
+
+
 @pytest.mark.parametrize("args, words", [
     (dict(budget=0), "budget"), (dict(budget=2.5), "budget"), (dict(budget=True), "budget"), (dict(budget=49), "budget"),
     (dict(budget=8, sinks=5, recent=4), "first"), (dict(budget=8, sinks=-1), "sinks"), (dict(budget=8, recent=-2), "recent"),
@@ -91,7 +99,7 @@ def test_c_entries_refuse_a_bad_cache(change):
     ("compact", dict(kept=None), -1), ("compact", dict(left=None), -1), ("compact", dict(left=8192), -1), ("compact", dict(budget=0), -1),
     ("select", dict(weight=None), -1), ("select", dict(budget=0), -1), ("select", dict(budget=64), -1), ("select", dict(sinks=5, recent=4), -1),
     ("select", dict(sinks=-1), -1), ("select", dict(batch=0), -1), ("select", dict(lens=12288), -1), ("select", dict(lens=12292), -1),
-    ("compact", dict(left=8196), -1), ("append", dict(counts=8196), -1), ("append", dict(at=8188), -1),
+    ("append", dict(T=(1 << 30) - 1), -1), ("compact", dict(left=8196), -1), ("append", dict(counts=8196), -1), ("append", dict(at=8188), -1),
 ])
 def test_c_entries_refuse_bad_arguments(entry, args, code):
     L = _lib.load()
