@@ -379,11 +379,14 @@ __global__ __launch_bounds__(kBlock) void cache_join_kernel(AttnArgs p, int D, i
 // ====================================================================================================================================
 // select: the tokens that stay
 // ====================================================================================================================================
-// One workgroup of 16 waves per (sequence, key head).  The r-th largest weight of the middle is found digit by digit (four passes of
-// eight bits over keys whose unsigned order is the weights' order).  Every wave has a stretch of tokens of its own, up to 2048 of them in
-// registers for all passes (longer stretches are read again); at the end it counts what stays of it, the counts are summed in wave order,
-// and it writes its kept indexes with ballots: ascending, and of equal weights the lowest indexes.
-constexpr int kSelBlock = 1024, kSelWaves = 16, kSelHeld = 32;
+// One workgroup of 16 waves per (sequence, key head).  The r-th largest weight of the middle is found digit by digit (up to four passes of
+// eight bits over keys whose unsigned order is the weights' order; three are enough where the weights differ in 24 bits).  Every wave has a
+// stretch of tokens of its own, up to 2048 of them in registers for all passes (longer stretches are read again); at the end it counts what
+// stays of it, the counts are summed in wave order, and it writes its kept indexes with ballots: ascending, and of equal weights the lowest
+// indexes.
+// Bound by the chain of its steps: 12 us for 4 352 weights of 128 rows (2.2 MB, 0.5 us at the rate of a copy), of which the launch and the
+// first loads take 6, a pass 1, counting and writing 1 each; 17 us for 12 755 of 16 rows.
+constexpr int kSelBlock = 1024, kSelWaves = 16, kSelHeld = 32, kSelCopies = 2;
 
 __device__ __forceinline__ unsigned weight_key(float w) {
     if (w != w) return 0u;   // a NaN counts less than every number
@@ -391,10 +394,22 @@ __device__ __forceinline__ unsigned weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// the sum over this lane and those below it: within rows of 16 lanes, then the rows' last sums into the rows above
+__device__ __forceinline__ unsigned upto_lane(unsigned x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 into rows 1 and 3, row_bcast 31 into 2 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+
 __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, const int* lens, int* kept, int* left, int kv, int cap, int budget,
                                                            int sinks, int recent) {
-    // counts by pass, in four copies a quarter of the lanes each (on different banks): weights share few values of the first digit
-    __shared__ __attribute__((aligned(16))) unsigned hist[4][4][256 + 16];
+    // counts by pass, in two copies of every other lane (on different banks): weights share few values of the first digit (two / four / eight
+    // copies 11.9 / 12.2 / 12.8 us with 4 352 tokens of 128 rows, 16.9 / 17.0 / 17.2 us with 12 755 of 16)
+    __shared__ __attribute__((aligned(16))) unsigned hist[4][kSelCopies][256 + 16];
     __shared__ int more[kSelWaves], same[kSelWaves];
     const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n = min(max(lens[b], 0), cap);
@@ -425,13 +440,13 @@ __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, 
     for (int i = tid; i < sinks; i += kSelBlock) out[i] = i;
     for (int i = tid; i < recent; i += kSelBlock) out[budget - recent + i] = m1 + i;
     if (need == 0) return;
-    for (int i = tid; i < 4 * 4 * 272; i += kSelBlock) (&hist[0][0][0])[i] = 0;
+    for (int i = tid; i < 4 * kSelCopies * 272; i += kSelBlock) (&hist[0][0][0])[i] = 0;
     __syncthreads();
     unsigned prefix = 0, mask = 0;
 #pragma unroll
     for (int pass = 0; pass < 4; ++pass) {
         const int shift = 24 - 8 * pass;
-        unsigned* mine = hist[pass][lane & 3];
+        unsigned* mine = hist[pass][lane & (kSelCopies - 1)];
         for (int from = w0; from < w1; from += kPart) {
             if (!once) fetch(from);
 #pragma unroll
@@ -444,30 +459,26 @@ __global__ __launch_bounds__(kSelBlock) void select_kernel(const float* weight, 
         // the digit at which the count from above reaches `need`: lane l holds digits 255 - 4 l down to 252 - 4 l
         unsigned c[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kSelCopies; ++k) {
             const u32x4 x = *reinterpret_cast<const u32x4*>(&hist[pass][k][252 - 4 * lane]);
             c[0] += x.w; c[1] += x.z; c[2] += x.y; c[3] += x.x;
         }
         const unsigned own = c[0] + c[1] + c[2] + c[3];
-        unsigned upto = own;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const unsigned x = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += x;
-        }
-        unsigned before = upto - own, digit = 0, rest = 0;
+        const unsigned upto = upto_lane(own);
+        unsigned before = upto - own, digit = 0, rest = 0, held_by = 0;
         const unsigned long long hit = __ballot(before < need && need <= upto);   // (one lane: at least `need` keys carry the prefix)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if (before < need && need <= before + c[k]) { digit = 255 - 4 * lane - k; rest = need - before; }
+            if (before < need && need <= before + c[k]) { digit = 255 - 4 * lane - k; rest = need - before; held_by = c[k]; }
             before += c[k];
         }
         const int from = __ffsll((long long)hit) - 1;
         prefix |= __builtin_amdgcn_readlane(digit, from) << shift;
         need = __builtin_amdgcn_readlane(rest, from);
         mask |= 255u << shift;
+        if (need == __builtin_amdgcn_readlane(held_by, from)) break;   // (all that carry the prefix stay: most often one, after three digits)
     }
-    // `prefix` is the smallest weight that stays, `need` of its equals stay with it
+    // nothing below `prefix` stays; of the weights that equal it the first `need`
     int a = 0, e = 0;
     for (int from = w0; from < w1; from += kPart) {
         if (!once) fetch(from);

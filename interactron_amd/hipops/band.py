@@ -68,7 +68,7 @@ class BandAttention(Function):
             lse = torch.empty(shape[0], shape[2], -(-shape[1] // 128) * 128, dtype=torch.float32, device=q.device)
             if q.dtype is not torch.float32:
                 rest = q.new_empty(shape)
-            ctx.how = (window, sinks, causal, scale)
+            ctx.how, ctx.band = (window, sinks, causal, scale), band
             ctx.save_for_backward(q, k, v, out, lse, rest, q_lens, kv_lens)
         ref, n, ws = ctypes.byref(band), ctypes.c_size_t(0), None
         _chk(_L().ix_workspace_bytes_band_attn_fwd(ref, ctypes.byref(n)), "ix_workspace_bytes_band_attn_fwd")
@@ -91,8 +91,10 @@ class BandAttention(Function):
             do = do.to(q.dtype)
         do = _dense_rows(do)
         s = _here(("the gradient",), do)
-        band = ctypes.byref(_band(q, k, v, q_lens, kv_lens, *ctx.how))
-        n = ctypes.c_size_t(0)
+        band = ctx.band
+        if (band.q, band.k, band.v, band.q_lens, band.kv_lens) != (q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_lens), _ptr(kv_lens)):
+            band = _band(q, k, v, q_lens, kv_lens, *ctx.how)   # (hooks have kept the saved tensors elsewhere)
+        band, n = ctypes.byref(band), ctypes.c_size_t(0)
         _chk(_L().ix_workspace_bytes_band_attn_bwd(band, ctypes.byref(n)), "ix_workspace_bytes_band_attn_bwd")
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)

@@ -229,6 +229,24 @@ def test_inputs_changed_in_between_are_noticed():
         out.backward(do)
 
 
+@TYPES
+def test_saved_tensors_kept_elsewhere(dtype):
+    """hooks that move what the forward pass saves: the gradients come from the tensors that come back"""
+    from interactron_amd import hipops
+    q, k, v, do = inputs(2, 150, 150, 4, 2, 64, dtype)
+    n = torch.tensor([150, 90], dtype=torch.int32, device="cuda")
+
+    def step():
+        t = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        return hipops.band_attention(*t, window=40, sinks=3, q_lens=n, kv_lens=n), t
+
+    out, t = step()
+    want = torch.autograd.grad(out, t, do)
+    with torch.autograd.graph.save_on_cpu():
+        out, t = step()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, t, do), want))
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_the_same_call_gives_the_same_bits(D):
     q, k, v, do = inputs(2, 700, 700, 8, 2, D, BF16)

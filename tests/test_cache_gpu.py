@@ -299,7 +299,7 @@ def test_select(budget, sinks, recent):
     check_select(w.cuda(), lens.cuda(), budget, sinks, recent)
 
 
-@pytest.mark.parametrize("kind", ["equal", "few", "negative", "special", "steps"])
+@pytest.mark.parametrize("kind", ["equal", "few", "negative", "special", "steps", "groups"])
 def test_select_ties_and_special_weights(kind):
     g = torch.Generator().manual_seed(3)
     shape = (3, 2, 5000)
@@ -312,6 +312,12 @@ def test_select_ties_and_special_weights(kind):
     elif kind == "special":
         pool = torch.tensor([float("nan"), float("inf"), float("-inf"), 0.0, -0.0, 1e-45, -1e-45, torch.finfo(FP32).max, torch.finfo(FP32).min, 1.0])
         w = pool[torch.randint(0, 10, shape, generator=g)]
+    elif kind == "groups":   # all weights of a size stay or go: 2999 and 700 of the large ones, alike in their first or first two digits
+        w = torch.rand(shape, generator=g) * 1e-3
+        for first, count, base in ((100, 700, 1.5), (1000, 2299, 1.0 + 2.0 ** -8)):
+            w[:, :, first: first + count] = base * (1 + torch.rand(3, 2, count, generator=g) * 2.0 ** -9)
+        for budget in (700, 2999, 3000, 2998):
+            check_select(w.cuda(), torch.tensor([5000, 4999, 3501], dtype=torch.int32, device="cuda"), budget, 0, 0)
     else:   # neighbours in the last bits
         w = (torch.randint(0, 1 << 12, shape, generator=g) + 0x3f800000).to(torch.int32).view(FP32)
     for budget, sinks, recent in ((700, 4, 100), (4999, 0, 0), (64, 0, 0), (3500, 10, 0)):
