@@ -342,6 +342,11 @@ constexpr float kFirstF = 1099511627776.f;   // 2^40
 // The running maximum is raised only where a tile exceeds it by more than 2^8 (a weight may then reach 256, exact in all types' ranges):
 // most tiles leave the accumulators alone.  16-bit types: a weight is rounded once to the type for the second product (half a step, like
 // the result itself: against 64 bits the two add up to sqrt(2) times the result's own rounding); the sum takes the unrounded weights.
+// Bound by matrix and vector instructions together (matrix pipe 43 % and vector instructions 51 % of busy cycles at hd 128, 33 and 63 % at hd 64, a
+// tenth of
+// the time for the bytes, no LDS conflicts): fp16, 8 192 queries and keys of 32 / 8 heads of 128, window 2 048: 275 us = 875 TFLOP/s, 0.75 of what a plain product
+// of 8 192^3 reaches; bf16, 12 755 of 8 heads of 64, window 2 551: 89-103 us = 580-680 TFLOP/s (at hd 64 a score costs as much exponential
+// for half the product); 2 060 of 16 heads of 64, window 412: 24 us, its 528 workgroups' first and last tiles.
 constexpr float kSlack = 8.f;
 
 template <int DT, int D, int NB, int TB>
@@ -490,6 +495,7 @@ __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) 
     }
 }
 
+// (the body is a device function: with it in the kernel, ROCm 7.2's host pass left the stubs of two blocks a wave undefined)
 template <int DT, int D, int NB>
 __global__ __launch_bounds__(kBlock, 2) void band_fwd_kernel(BandArgs a) {
     constexpr int STAGE = 2 * key_tile(DT) * Img<DT, D>::ROW;
@@ -497,7 +503,7 @@ __global__ __launch_bounds__(kBlock, 2) void band_fwd_kernel(BandArgs a) {
     band_fwd<DT, D, NB, key_tile(DT)>(a, mem);
 }
 
-// The pieces of every row joined, in their order, four values a lane.
+// The pieces of every row joined, in their order, four values a lane: 5 us for 640 rows of 128 in 23 pieces (7.6 MB), 12 with one piece at a time.
 template <int DT, int D>
 __global__ __launch_bounds__(kBlock) void band_join_kernel(BandArgs a) {
     constexpr int LANES = D / 4;
@@ -510,12 +516,30 @@ __global__ __launch_bounds__(kBlock) void band_join_kernel(BandArgs a) {
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     if (i < a.m(b)) {
         const int64_t at = (bh * a.Lq + i) * a.fwd_splits;
-        for (int s = 0; s < a.fwd_splits; ++s) {
-            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (at + s));
-            const f32x4 o = *reinterpret_cast<const f32x4*>(a.part + (at + s) * D + 4 * c);
-            const float up = fmaxf(top, ml.x), ref = up == -INFINITY ? 0.f : up, f0 = seq_exp2(top - ref), f1 = seq_exp2(ml.x - ref);
-            sum = sum * f0 + ml.y * f1;
-            x = x * f0 + o * f1;
+        for (int s0 = 0; s0 < a.fwd_splits; s0 += 8) {   // eight pieces' loads in flight
+            float2 ml[8];
+            f32x4 o[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int s = min(s0 + u, a.fwd_splits - 1);
+                ml[u] = *reinterpret_cast<const float2*>(a.part_ml + 2 * (at + s));
+                o[u] = *reinterpret_cast<const f32x4*>(a.part + (at + s) * D + 4 * c);
+            }
+            float up = top;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                ml[u].x = s0 + u < a.fwd_splits ? ml[u].x : -INFINITY;
+                up = fmaxf(up, ml[u].x);
+            }
+            const float ref = up == -INFINITY ? 0.f : up, down = seq_exp2(top - ref);
+            sum *= down;
+            x *= down;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float f = seq_exp2(ml[u].x - ref);
+                sum += ml[u].y * f;
+                x += o[u] * f;
+            }
             top = up;
         }
     }
@@ -526,8 +550,9 @@ __global__ __launch_bounds__(kBlock) void band_join_kernel(BandArgs a) {
 // ====================================================================================================================================
 // gradients
 // ====================================================================================================================================
-// -delta_i = -do_i o_i (where the sums of do_i v_j start), a row by the lanes that hold 16 bytes of it each.  16-bit: o is the stored output and the rest its rounding took, so
-// that delta -- which is subtracted from every do_i v_j of the row -- is as good as from the 32-bit output.
+// -delta_i = -do_i o_i (where the sums of do_i v_j start), a row by the lanes that hold 16 bytes of it each.  16-bit: o is the stored output and
+// the rest its rounding took, so that delta -- which is subtracted from every do_i v_j of the row -- is as good as from the 32-bit output.
+// HBM-bound, with a launch's few microseconds before it: 102 040 rows of 64 in bf16 8 us, 4.9 TB/s.
 template <int DT, int D>
 __global__ __launch_bounds__(kBlock) void band_delta_kernel(BandArgs a) {
     constexpr int EB = SeqT<DT>::bytes, LANES = D * EB / 16;
@@ -877,6 +902,10 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
 }
 
 // Both in one launch, the key blocks first: either alone would leave compute units empty at the sizes where time counts, and at its end.
+// Nine products of 2 hd operations a pair (four of the formulas, q k^T and do v^T twice, the second terms of dz): 12 755 queries and keys of 8
+// heads of 64, window 2 551, bf16: 307-343 us = 790-900 TFLOP/s, matrix pipe 43 % and vector instructions 56 % of busy cycles; head dim 128 at
+// 8 192 of 32 / 8 heads, window 2 048: 1 317 us = 820 TFLOP/s; f32, 16 x 361 of 8 heads of 32, window 64: 47 us.  Scores of the next 32 rows
+// ahead of this one's exponentials: 350 / 350 us.
 template <int DT, int D> constexpr int bwd_bytes() {
     constexpr int qs = 2 * key_tile(DT) * Img<DT, D>::ROW, ks = 2 * query_tile(DT, D) * Img<DT, D>::ROW;
     constexpr int q = stages(qs) * qs, k = stages(ks) * (ks + 1024);
