@@ -191,8 +191,11 @@ template <int N> __device__ __forceinline__ void landed() {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
-// stages of the ring: three (requests two tiles ahead) where a workgroup's LDS stays within 48 KB, else two
-constexpr int stages(int bytes) { return 3 * bytes <= 49152 ? 3 : 2; }
+// stages of the ring: three (requests two tiles ahead) where a workgroup's LDS stays within the limit, else two.  Gradients 48 KB; forward 32,
+// where one more workgroup fits on a compute unit instead (48 / 32 KB: f32 of 8 heads of 64, 8 192 with window 1 000 173 / 161 us; bf16, 12 755
+// with window 2 551 102 / 99.5, 2 x 2 060 with window 412 22.7 / 22.1, 2 x 4 096 in full 62.5 / 64).
+constexpr int stages(int bytes, int limit) { return 3 * bytes <= limit ? 3 : 2; }
+constexpr int kFwdRing = 32768, kBwdRing = 49152;
 
 struct BandArgs {
     const unsigned char *q, *k, *v, *go, *o, *o_rest;
@@ -342,17 +345,16 @@ constexpr float kFirstF = 1099511627776.f;   // 2^40
 // The running maximum is raised only where a tile exceeds it by more than 2^8 (a weight may then reach 256, exact in all types' ranges):
 // most tiles leave the accumulators alone.  16-bit types: a weight is rounded once to the type for the second product (half a step, like
 // the result itself: against 64 bits the two add up to sqrt(2) times the result's own rounding); the sum takes the unrounded weights.
-// Bound by matrix and vector instructions together (matrix pipe 43 % and vector instructions 51 % of busy cycles at hd 128, 33 and 63 % at hd 64, a
-// tenth of
-// the time for the bytes, no LDS conflicts): fp16, 8 192 queries and keys of 32 / 8 heads of 128, window 2 048: 275 us = 875 TFLOP/s, 0.75 of what a plain product
-// of 8 192^3 reaches; bf16, 12 755 of 8 heads of 64, window 2 551: 89-103 us = 580-680 TFLOP/s (at hd 64 a score costs as much exponential
-// for half the product); 2 060 of 16 heads of 64, window 412: 24 us, its 528 workgroups' first and last tiles.
+// Bound by matrix and vector instructions together (matrix pipe 43 % and vector instructions 51 % of busy cycles at hd 128, 33 and 63 % at
+// hd 64, a tenth of the time for the bytes, no LDS conflicts): fp16, 8 192 queries and keys of 32 / 8 heads of 128, window 2 048: 275 us =
+// 875 TFLOP/s, 0.75 of what a plain product of 8 192^3 reaches; bf16, 12 755 of 8 heads of 64, window 2 551: 89-103 us = 580-680 TFLOP/s (a
+// score costs as much exponential for half the product); 2 060 of 16 heads of 64, window 412: 24 us, its 528 workgroups' first and last tiles.
 constexpr float kSlack = 8.f;
 
 template <int DT, int D, int NB, int TB>
 __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) {
     typedef Img<DT, D> I;
-    constexpr int ROWS = 16 * NB * kWaves, SB = TB / 16, BYTES = TB * I::ROW, STG = stages(2 * BYTES);
+    constexpr int ROWS = 16 * NB * kWaves, SB = TB / 16, BYTES = TB * I::ROW, STG = stages(2 * BYTES, kFwdRing);
     auto lds = reinterpret_cast<unsigned char (*)[2][BYTES]>(mem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
     const int bh = spread_heads(blockIdx.x, a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.kv);
@@ -499,7 +501,7 @@ __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) 
 template <int DT, int D, int NB>
 __global__ __launch_bounds__(kBlock, 2) void band_fwd_kernel(BandArgs a) {
     constexpr int STAGE = 2 * key_tile(DT) * Img<DT, D>::ROW;
-    __shared__ __attribute__((aligned(256))) unsigned char mem[stages(STAGE) * STAGE];
+    __shared__ __attribute__((aligned(256))) unsigned char mem[stages(STAGE, kFwdRing) * STAGE];
     band_fwd<DT, D, NB, key_tile(DT)>(a, mem);
 }
 
@@ -585,7 +587,7 @@ __global__ __launch_bounds__(kBlock) void band_delta_kernel(BandArgs a) {
 template <int DT, int D, int NB, int TB>
 __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, int group) {
     typedef Img<DT, D> I;
-    constexpr int ROWS = 16 * NB * kWaves, BYTES = TB * I::ROW, STG = stages(2 * BYTES);
+    constexpr int ROWS = 16 * NB * kWaves, BYTES = TB * I::ROW, STG = stages(2 * BYTES, kBwdRing);
     auto lds = reinterpret_cast<unsigned char (*)[2][BYTES]>(mem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
     const int bh = spread_heads(group % (a.B * a.H), a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.kv);
@@ -737,7 +739,7 @@ struct KeyItem {
 template <int DT, int D, int NB, int TB>
 __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, int group) {
     typedef Img<DT, D> I;
-    constexpr int ROWS = 16 * NB * kWaves, BYTES = TB * I::ROW, STG = stages(2 * BYTES);
+    constexpr int ROWS = 16 * NB * kWaves, BYTES = TB * I::ROW, STG = stages(2 * BYTES, kBwdRing);
     auto lds = reinterpret_cast<unsigned char (*)[2][BYTES]>(mem);
     auto row_c = reinterpret_cast<float (*)[4][64]>(mem + STG * 2 * BYTES);   // lse, -delta of the tile's queries (and what waves 2, 3 fetch)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
@@ -908,7 +910,7 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
 // ahead of this one's exponentials: 350 / 350 us.
 template <int DT, int D> constexpr int bwd_bytes() {
     constexpr int qs = 2 * key_tile(DT) * Img<DT, D>::ROW, ks = 2 * query_tile(DT, D) * Img<DT, D>::ROW;
-    constexpr int q = stages(qs) * qs, k = stages(ks) * (ks + 1024);
+    constexpr int q = stages(qs, kBwdRing) * qs, k = stages(ks, kBwdRing) * (ks + 1024);
     return q > k ? q : k;
 }
 template <int DT, int D, int NB>
