@@ -4,7 +4,7 @@ The sliding form of hipops.attention for rollouts that are too long to attend to
 models/detr_models/transformer.py:148-161 attend to everything): 16-bit or 32-bit rows as they are, shared key heads, padded batches.
 """
 import ctypes
-import math
+import struct
 
 import torch
 
@@ -13,12 +13,8 @@ from .cache import _DTYPES, _HEAD_DIMS, _count, _here
 from .core import Function, _L, _NullCtx, _chk
 
 
-class _BandC(ctypes.Structure):   # struct ix_band of include/interactron_hip.h
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v")] +
-                [("%s_s%s" % (t, d), ctypes.c_int64) for t in "qkv" for d in "blh"] +
-                [("q_lens", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p)] +
-                [(n, ctypes.c_int) for n in ("dtype", "batch", "Lq", "Lk", "heads", "kv_heads", "hd", "window", "sinks", "causal")] +
-                [("scale", ctypes.c_float)])
+# struct ix_band of include/interactron_hip.h: q, k, v, nine strides, q_lens, kv_lens, dtype .. causal, scale
+_pack = struct.Struct("3P9q2P10if4x").pack
 
 
 _NAMES = ("q", "k", "v", "q_lens", "kv_lens")
@@ -38,13 +34,17 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _band(q, k, v, q_lens, kv_lens, window, sinks, causal, scale):
     B, Lq, H, D = q.shape
     qb, ql, qh, _ = q.stride()
     kb, kl, kh, _ = k.stride()
     vb, vl, vh, _ = v.stride()
-    return _BandC(q.data_ptr(), k.data_ptr(), v.data_ptr(), qb, ql, qh, kb, kl, kh, vb, vl, vh, _ptr(q_lens), _ptr(kv_lens),
-                  _DTYPES[q.dtype], B, Lq, k.shape[1], H, k.shape[2], D, window, sinks, causal, scale)
+    return _pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), qb, ql, qh, kb, kl, kh, vb, vl, vh, 0 if q_lens is None else q_lens.data_ptr(),
+                 0 if kv_lens is None else kv_lens.data_ptr(), _DTYPES[q.dtype], B, Lq, k.shape[1], H, k.shape[2], D, window, sinks, causal, scale)
 
 
 class BandAttention(Function):
@@ -63,20 +63,19 @@ class BandAttention(Function):
             return q.new_zeros(shape)
         q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
         band = _band(q, k, v, q_lens, kv_lens, window, sinks, causal, scale)
-        out, lse, rest = q.new_empty(shape), None, None
-        if recorded:   # the rows' normalisers and, with 16-bit types, what rounding took from the output: for the gradients
-            lse = torch.empty(shape[0], shape[2], -(-shape[1] // 128) * 128, dtype=torch.float32, device=q.device)
-            if q.dtype is not torch.float32:
-                rest = q.new_empty(shape)
-            ctx.how, ctx.band = (window, sinks, causal, scale), band
-            ctx.save_for_backward(q, k, v, out, lse, rest, q_lens, kv_lens)
-        ref, n, ws = ctypes.byref(band), ctypes.c_size_t(0), None
-        _chk(_L().ix_workspace_bytes_band_attn_fwd(ref, ctypes.byref(n)), "ix_workspace_bytes_band_attn_fwd")
+        out, lse, rest = _like(q), None, None
+        if recorded:   # for the gradients: the rows' normalisers and, with 16-bit types, behind them what rounding took from the output
+            n = shape[0] * shape[2] * (-(-shape[1] // 128) * 512)
+            kept = torch.empty(n if q.dtype is torch.float32 else n + 2 * q.numel(), dtype=torch.uint8, device=q.device)
+            lse = kept.data_ptr()
+            rest = None if q.dtype is torch.float32 else lse + n
+            ctx.how = (window, sinks, causal, scale)
+            ctx.save_for_backward(q, k, v, out, kept, q_lens, kv_lens)
+        n, ws = ctypes.c_size_t(0), None
+        _chk(_L().ix_workspace_bytes_band_attn_fwd(band, ctypes.byref(n)), "ix_workspace_bytes_band_attn_fwd")
         if n.value:
             ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        rc = _L().ix_band_attn_fwd(ref, out.data_ptr(), _ptr(lse), _ptr(rest), _ptr(ws), n.value, s)
-        if rc:
-            _chk(rc, "ix_band_attn_fwd")
+        _chk(_L().ix_band_attn_fwd(band, out.data_ptr(), lse, rest, _ptr(ws), n.value, s), "ix_band_attn_fwd")
         return out
 
     @staticmethod
@@ -86,23 +85,19 @@ class BandAttention(Function):
         need = ctx.needs_input_grad
         if ctx.empty:
             return tuple([torch.zeros_like(t) if n else None for t, n in zip(ctx.saved_tensors, need)]) + (None,) * 6
-        q, k, v, out, lse, rest, q_lens, kv_lens = ctx.saved_tensors
+        q, k, v, out, kept, q_lens, kv_lens = ctx.saved_tensors
         if do.dtype is not q.dtype:
             do = do.to(q.dtype)
         do = _dense_rows(do)
         s = _here(("the gradient",), do)
-        band = ctx.band
-        if (band.q, band.k, band.v, band.q_lens, band.kv_lens) != (q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_lens), _ptr(kv_lens)):
-            band = _band(q, k, v, q_lens, kv_lens, *ctx.how)   # (hooks have kept the saved tensors elsewhere)
-        band, n = ctypes.byref(band), ctypes.c_size_t(0)
+        band, n = _band(q, k, v, q_lens, kv_lens, *ctx.how), ctypes.c_size_t(0)
         _chk(_L().ix_workspace_bytes_band_attn_bwd(band, ctypes.byref(n)), "ix_workspace_bytes_band_attn_bwd")
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        gb, gl, gh, _ = do.stride()
-        rc = _L().ix_band_attn_bwd(band, out.data_ptr(), _ptr(rest), lse.data_ptr(), do.data_ptr(), gb, gl, gh, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                   ws.data_ptr(), n.value, s)
-        if rc:
-            _chk(rc, "ix_band_attn_bwd")
+        dq, dk, dv = _like(q), _like(k), _like(v)
+        lse, (gb, gl, gh, _) = kept.data_ptr(), do.stride()
+        rest = None if q.dtype is torch.float32 else lse + kept.numel() - 2 * q.numel()
+        _chk(_L().ix_band_attn_bwd(band, out.data_ptr(), rest, lse, do.data_ptr(), gb, gl, gh, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(),
+                                   n.value, s), "ix_band_attn_bwd")
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None, None, None
 
 
@@ -135,6 +130,6 @@ def band_attention(q, k, v, window=None, sinks=0, causal=True, scale=None, q_len
             raise ValueError("%s must be a contiguous int32 [%d], got %s %s" % (name, B, t.dtype, list(t.shape)))
     window, sinks = 0 if window is None else _count(window, "window", 1), _count(sinks, "sinks")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
+    if not abs(scale) < 3e38:   # (a float32, and no NaN)
         raise ValueError("scale must be a finite number, got %r" % scale)
     return BandAttention.call(q, k, v, q_lens, kv_lens, window, sinks, 1 if causal else 0, scale)

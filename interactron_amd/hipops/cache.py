@@ -11,7 +11,6 @@ alone (the lengths stay on the device) and may be captured into a HIP graph.  (T
 over all frames again for every new one, models/interactron.py:166-190.)
 """
 import ctypes
-import math
 
 import torch
 
@@ -195,7 +194,7 @@ def cache_attention(q, cache, scale=None, window=None, sinks=0, accumulate=False
     if accumulate and cache.weight is None:
         raise ValueError("accumulate: the cache holds no weights")
     scale = cache.hd ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
+    if not abs(scale) < 3e38:   # (a float32, and no NaN)
         raise ValueError("scale must be a finite number, got %r" % scale)
     s = _here(("q",), q)
     out, ws, need = q.new_empty(shape), None, _attention_ws(cache, H, w, sinks, accumulate)

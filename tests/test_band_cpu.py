@@ -21,7 +21,7 @@ def test_cpu_tensors_are_refused():
 @pytest.mark.parametrize("shape, how, words", [
     (dict(D=48), {}, "head dim of 48"), (dict(H=3), {}, "3 query heads"), (dict(kv=0), {}, "key heads"), (dict(dtype=torch.float64), {}, "q must be"),
     ({}, dict(window=0), "window"), ({}, dict(window=-3), "window"), ({}, dict(window=1.5), "window"), ({}, dict(window=1 << 30), "window"),
-    ({}, dict(sinks=-1), "sinks"), ({}, dict(sinks=None), "sinks"), ({}, dict(scale=float("nan")), "scale"), ({}, dict(scale=float("inf")), "scale"),
+    ({}, dict(sinks=-1), "sinks"), ({}, dict(sinks=None), "sinks"), ({}, dict(scale=float("nan")), "scale"), ({}, dict(scale=float("inf")), "scale"), ({}, dict(scale=-1e39), "scale"),
     ({}, dict(q_lens=torch.zeros(2)), "q_lens"), ({}, dict(kv_lens=torch.zeros(3, dtype=torch.int32)), "kv_lens"),
     ({}, dict(kv_lens=torch.zeros(4, dtype=torch.int32)[::2]), "kv_lens"), ({}, dict(q_lens=torch.zeros(2, dtype=torch.int64)), "q_lens"),
 ])
@@ -43,12 +43,30 @@ def test_tensors_that_do_not_fit_are_refused(change):
         hipops.band_attention(*change(*qkv()))
 
 
+class BandC(ctypes.Structure):   # struct ix_band of include/interactron_hip.h
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v")] + [("%s_s%s" % (t, d), ctypes.c_int64) for t in "qkv" for d in "blh"] +
+                [("q_lens", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p)] +
+                [(n, ctypes.c_int) for n in ("dtype", "batch", "Lq", "Lk", "heads", "kv_heads", "hd", "window", "sinks", "causal")] +
+                [("scale", ctypes.c_float)])
+
+
 def c_band(**change):
     """A description whose pointers are never followed"""
     f = dict(q=4096, k=4096, v=4096, q_sb=1280, q_sl=256, q_sh=64, k_sb=896, k_sl=128, k_sh=64, v_sb=896, v_sl=128, v_sh=64, q_lens=None, kv_lens=None,
              dtype=1, batch=2, Lq=5, Lk=7, heads=4, kv_heads=2, hd=64, window=0, sinks=0, causal=1, scale=0.125)
     f.update(change)
-    return hipops.band._BandC(*[f[n] for n, _ in hipops.band._BandC._fields_])
+    return BandC(*[f[n] for n, _ in BandC._fields_])
+
+
+def test_the_description_is_packed_as_the_header_lays_it_out():
+    q, k, v = torch.zeros(2, 5, 4, 64, dtype=BF16), torch.zeros(2, 7, 2, 64, dtype=BF16), torch.zeros(2, 7, 4, 64, dtype=BF16)[:, :, :2]
+    n = torch.zeros(2, dtype=torch.int32)
+    for lens in (None, n):
+        c = BandC.from_buffer_copy(hipops.band._band(q, k, v, n, lens, 3, 9, 1, -0.25))
+        want = dict(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_sb=1280, q_sl=256, q_sh=64, k_sb=896, k_sl=128, k_sh=64, v_sb=1792, v_sl=256, v_sh=64,
+                    q_lens=n.data_ptr(), kv_lens=None if lens is None else n.data_ptr(), dtype=1, batch=2, Lq=5, Lk=7, heads=4, kv_heads=2, hd=64, window=3,
+                    sinks=9, causal=1, scale=-0.25)
+        assert {f: getattr(c, f) for f, _ in BandC._fields_} == want
 
 
 @pytest.mark.parametrize("change", [dict(q=None), dict(k=None), dict(v=4100), dict(dtype=3), dict(hd=80), dict(batch=0), dict(Lq=0), dict(Lk=0), dict(Lq=65535 * 64 + 1), dict(Lk=65535 * 64 + 1),
