@@ -201,10 +201,11 @@ struct BandArgs {
     const unsigned char *q, *k, *v, *go, *o, *o_rest;
     int64_t qb, ql, qh, kb, kl, kh, vb, vl, vh, gb, gl, gh;   // bytes
     unsigned char *out, *rest, *dq, *dk, *dv;                 // dense; rest: what rounding the output to 16 bits took away, in 16 bits
-    float *lse, *delta, *part, *part_ml;                      // [B][H][Lp] base-2 normalisers (+inf: nothing visible) and delta; partial sums
+    float *lse, *delta, *part, *part_ml, *part_q;             // [B][H][Lp] base-2 normalisers (+inf: nothing visible) and delta; partial sums
     const int *q_lens, *kv_lens;
     int B, Lq, Lk, Lp, H, kv, left, right, sinks, causal;
     int wide_blocks, wide_splits, splits, key_groups;         // dk / dv: see the host side; workgroups of theirs
+    int q_splits;                                             // dq: pieces of a block's key tiles
     int fwd_splits;                                           // forward: pieces of a block's key tiles
     float c2, scale;                                          // |scale| log2(e), scale
     unsigned flip;                                            // sign bits of a fragment's register where scale < 0
@@ -583,7 +584,8 @@ __global__ __launch_bounds__(kBlock) void band_delta_kernel(BandArgs a) {
     if (c == 0) a.delta[((int64_t)b * a.H + h) * a.Lp + i] = -d;
 }
 
-// dq: query-owning, streams k (both ways) and v (rows).  Tiles are taken 32 keys at a time.
+// dq: query-owning, streams k (both ways) and v (rows).  Tiles are taken 32 keys at a time.  Pieces of a block's tiles leave f32 partial sums
+// [ROWS][D]; band_sum_kernel adds them in order.
 template <int DT, int D, int NB, int TB>
 __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, int group) {
     typedef Img<DT, D> I;
@@ -591,7 +593,8 @@ __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, i
     auto lds = reinterpret_cast<unsigned char (*)[2][BYTES]>(mem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
     const int bh = spread_heads(group % (a.B * a.H), a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.kv);
-    const int blocks = (a.Lq + ROWS - 1) / ROWS, y = group / (a.B * a.H), i0 = (a.causal ? blocks - 1 - y : y) * ROWS;
+    const int piece = group / (a.B * a.H), split = piece % a.q_splits, y = piece / a.q_splits;
+    const int blocks = (a.Lq + ROWS - 1) / ROWS, blk = a.causal ? blocks - 1 - y : y, i0 = blk * ROWS;
     const int m = a.m(b), n = a.n(b), shift = n - m, iw = i0 + wave * 16 * NB;
     f32x4 acc[NB][I::DB];
     float lse[NB], delta[NB], F[NB];
@@ -624,15 +627,16 @@ __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, i
             dk.issue(lds[st][0], wave, row0, n);
             dv.issue(lds[st][1], wave, row0, n);
         };
+        const int t0 = kt.count * split / a.q_splits, t1 = kt.count * (split + 1) / a.q_splits;
 #pragma unroll
         for (int t = 0; t < STG - 1; ++t)
-            if (t < kt.count) issue(t);
-        for (int t = 0; t < kt.count; ++t) {
+            if (t0 + t < t1) issue(t0 + t);
+        for (int t = t0; t < t1; ++t) {
             const unsigned char *ki = lds[t % STG][0], *vi = lds[t % STG][1];
             const int j0 = kt.tile(t) * TB;
-            if (STG == 3 && t + 1 < kt.count) landed<2 * Dma<DT, D, TB>::N>();
+            if (STG == 3 && t + 1 < t1) landed<2 * Dma<DT, D, TB>::N>();
             else landed<0>();
-            if (t + STG - 1 < kt.count) issue(t + STG - 1);
+            if (t + STG - 1 < t1) issue(t + STG - 1);
             if (iw < m && !a.none_sees(pw0, pw1, j0, j0 + TB - 1)) {
                 const bool part = j0 + TB > n || !a.all_see(pw0, pw1, j0, j0 + TB - 1);
 #pragma unroll
@@ -714,8 +718,14 @@ __device__ __forceinline__ void band_dq(const BandArgs& a, unsigned char* mem, i
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const int i = iw + 16 * nb + n16;
-        if (i >= a.Lq) continue;
         const float f = DT == 2 ? a.scale / F[nb] : a.scale;
+        if (a.q_splits > 1) {
+            float* dst = a.part_q + ((((int64_t)bh * blocks + blk) * a.q_splits + split) * ROWS + i - i0) * D;
+#pragma unroll
+            for (int db = 0; db < I::DB; ++db) *reinterpret_cast<f32x4*>(dst + 16 * db + 4 * g) = acc[nb][db] * f;
+            continue;
+        }
+        if (i >= a.Lq) continue;
         unsigned char* dst = a.dq + (((int64_t)b * a.Lq + i) * a.H + h) * I::ROW;
 #pragma unroll
         for (int db = 0; db < I::DB; ++db) store4<DT>(dst + (16 * db + 4 * g) * I::EB, acc[nb][db] * f);
@@ -920,20 +930,36 @@ __global__ __launch_bounds__(kBlock, 2) void band_bwd_kernel(BandArgs a) {
     else band_dq<DT, D, NB, key_tile(DT)>(a, mem, blockIdx.x - a.key_groups);
 }
 
-// dk, dv of the blocks that were cut into splits: the partial sums in split order, four values a thread
+// dk, dv (and, with pieces of dq, then dq) of the blocks that were cut: the partial sums in their order, four values a thread
 template <int DT, int D>
 __global__ __launch_bounds__(kBlock) void band_sum_kernel(BandArgs a, int items, int rows) {
     typedef Img<DT, D> I;
+    const int block = blockIdx.y;
+    if ((int)blockIdx.x >= a.B * a.kv) {
+        const int bh = blockIdx.x - a.B * a.kv, b = bh / a.H, h = bh % a.H, blocks = (a.Lq + rows - 1) / rows;
+        if (block >= blocks) return;
+        for (int e = (blockIdx.z * kBlock + threadIdx.x) * 4; e < rows * D; e += gridDim.z * kBlock * 4) {
+            const int i = block * rows + e / D;
+            if (i >= a.Lq) continue;
+            const float* src = a.part_q + ((int64_t)bh * blocks + block) * a.q_splits * rows * D + e;
+            f32x4 x = *reinterpret_cast<const f32x4*>(src);
+#pragma unroll 8
+            for (int s = 1; s < a.q_splits; ++s) x += *reinterpret_cast<const f32x4*>(src + (int64_t)s * rows * D);
+            store4<DT>(a.dq + (((int64_t)b * a.Lq + i) * a.H + h) * I::ROW + e % D * I::EB, x);
+        }
+        return;
+    }
     const int bk = blockIdx.x, b = bk / a.kv, hk = bk % a.kv;
-    const bool wide = (int)blockIdx.y < a.wide_blocks;
+    const bool wide = block < a.wide_blocks;
     const int splits = wide ? a.wide_splits : a.splits;
-    if (splits == 1) return;
-    const int block = blockIdx.y, item = wide ? block * splits : a.wide_blocks * a.wide_splits + (block - a.wide_blocks) * splits;
+    if (splits == 1 || (int64_t)block * rows >= a.Lk) return;
+    const int item = wide ? block * splits : a.wide_blocks * a.wide_splits + (block - a.wide_blocks) * splits;
     for (int e = (blockIdx.z * kBlock + threadIdx.x) * 4; e < 2 * rows * D; e += gridDim.z * kBlock * 4) {
         const int which = e / (rows * D), row = e / D % rows, d = e % D, j = block * rows + row;
         if (j >= a.Lk) continue;
         const float* src = a.part + ((int64_t)bk * items + item) * 2 * rows * D + e;
         f32x4 x = *reinterpret_cast<const f32x4*>(src);
+#pragma unroll 8
         for (int s = 1; s < splits; ++s) x += *reinterpret_cast<const f32x4*>(src + (int64_t)s * 2 * rows * D);
         store4<DT>((which ? a.dv : a.dk) + (((int64_t)b * a.Lk + j) * a.kv + hk) * I::ROW + d * I::EB, x);
     }
@@ -982,7 +1008,10 @@ struct KeyPlan { int blocks, wide, wide_splits, splits, items; };
 
 // Splits of dk / dv.  A block of keys streams the queries of its band; a block with some of the first `sinks` keys streams all of them, and
 // where these are more than two and a half times the others' it would run on alone: it is cut into pieces of up to twice the others'
-// length.  Where all blocks together are fewer than the compute units (few key heads, many query heads), every block is cut.
+// length.  Where all blocks together are fewer than the compute units (few key heads, many query heads), every block is cut, into about 384
+// pieces in all: forward and gradients with 256 / 384 / 512 for the keys and for dq, f32, 2 x 2 041 of 2 heads of 64 180 / 146 / 145 us, 6 000 of
+// one head of 128 580 / 437 / 453; bf16, 6 000 of 2 heads of 64 169 / 143 / 142, 40 queries of 16 heads over 6 000 keys of 4 of 128 58 / 57 / 68.
+// With 264 blocks (2 060 of 8 heads, every key) two pieces each cost 5 us more than none.
 KeyPlan key_plan(const ix_band* s) {
     KeyPlan r;
     const int rows = owner_rows(bwd_nb(s)), group = s->heads / s->kv_heads, tb = query_tile(s->dtype, s->hd);
@@ -990,7 +1019,7 @@ KeyPlan key_plan(const ix_band* s) {
     r.wide = s->sinks > 0 ? (s->sinks < s->Lk ? (int)div_up(s->sinks, rows) : r.blocks) : 0;
     const int64_t all = div_up(s->Lq, tb), band = div_up(reach(s) + rows, tb) + 1, each = (band < all ? band : all) * group;
     const int64_t wgs = (int64_t)s->batch * s->kv_heads * r.blocks;
-    int64_t sp = wgs < 256 ? div_up(256, wgs) : 1;
+    int64_t sp = wgs < 256 ? div_up(384, wgs) : 1;
     if (sp > div_up(each, 4)) sp = div_up(each, 4);   // (no piece under four tiles)
     r.splits = (int)(sp < 1 ? 1 : sp);
     const int64_t piece = div_up(each, r.splits);
@@ -1001,6 +1030,22 @@ KeyPlan key_plan(const ix_band* s) {
     r.wide_splits = (int)(ws > 64 ? 64 : ws);
     r.items = r.wide * r.wide_splits + (r.blocks - r.wide) * r.splits;
     return r;
+}
+
+// Pieces of dq's key tiles, by the same rule as the keys' blocks: at least four tiles each, where the blocks of queries are fewer than the
+// compute units (uncut: 40 queries of 16 heads over 6 000 keys 159 us instead of 58, 6 000 of one head of 128 in f32 977 instead of 580).
+int dq_splits(const ix_band* s) {
+    const int64_t groups = (int64_t)s->batch * s->heads * div_up(s->Lq, owner_rows(bwd_nb(s)));
+    if (groups >= 256) return 1;
+    const int tb = key_tile(s->dtype);
+    const int64_t all = div_up(s->Lk, tb), some = div_up(reach(s) + owner_rows(bwd_nb(s)), tb) + 1 + div_up(s->sinks, tb), tiles = some < all ? some : all;
+    int64_t r = div_up(384, groups);
+    if (r > tiles / 4) r = tiles / 4;
+    return (int)(r < 2 ? 1 : r > 32 ? 32 : r);
+}
+size_t dq_part_bytes(const ix_band* s) {
+    const int r = dq_splits(s), rows = owner_rows(bwd_nb(s));
+    return r == 1 ? 0 : (size_t)s->batch * s->heads * div_up(s->Lq, rows) * r * rows * s->hd * 4;
 }
 
 size_t part_bytes(const ix_band* s, const KeyPlan& r) {
@@ -1114,7 +1159,7 @@ extern "C" int ix_workspace_bytes_band_attn_bwd(const struct ix_band* s, size_t*
     BandArgs a;
     if (int rc = band_of(a, s, "ix_workspace_bytes_band_attn_bwd")) return rc;
     IX_CHECK_ARG(out_host, "ix_workspace_bytes_band_attn_bwd: null output");
-    *out_host = (size_t)a.B * a.H * a.Lp * 4 + part_bytes(s, key_plan(s));
+    *out_host = (size_t)a.B * a.H * a.Lp * 4 + part_bytes(s, key_plan(s)) + dq_part_bytes(s);
     return IX_OK;
 }
 
@@ -1128,7 +1173,7 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
     for (int64_t x : {g_sb, g_sl, g_sh}) IX_CHECK_ARG(x * eb % 16 == 0, "ix_band_attn_bwd: rows that do not start on 16 bytes");
     IX_CHECK_ARG(g_sl >= 0 && g_sl * eb < (1 << 24), "ix_band_attn_bwd: rows 2^24 bytes apart or more");
     const KeyPlan r = key_plan(s);
-    const size_t parts = part_bytes(s, r), need = (size_t)a.B * a.H * a.Lp * 4 + parts;
+    const size_t parts = part_bytes(s, r), parts_q = dq_part_bytes(s), need = (size_t)a.B * a.H * a.Lp * 4 + parts + parts_q;
     if (!workspace || workspace_bytes < need || !ix_al16(workspace)) {
         ix_set_error("ix_band_attn_bwd: workspace of %zu bytes (16-byte aligned), %zu needed", workspace ? workspace_bytes : (size_t)0, need);
         return IX_ERR_WORKSPACE;
@@ -1140,6 +1185,8 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
     a.lse = const_cast<float*>(lse);
     a.delta = static_cast<float*>(workspace);
     a.part = a.delta + (size_t)a.B * a.H * a.Lp;
+    a.part_q = a.part + parts / 4;
+    a.q_splits = dq_splits(s);
     a.dq = static_cast<unsigned char*>(dq);
     a.dk = static_cast<unsigned char*>(dk);
     a.dv = static_cast<unsigned char*>(dv);
@@ -1147,7 +1194,7 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
     a.wide_splits = r.wide_splits;
     a.splits = r.splits;
     const int nb = bwd_nb(s), rows = owner_rows(nb);
-    const int64_t key_groups = (int64_t)a.B * a.kv * r.items, groups = key_groups + (int64_t)a.B * a.H * ((a.Lq + rows - 1) / rows);
+    const int64_t key_groups = (int64_t)a.B * a.kv * r.items, groups = key_groups + (int64_t)a.B * a.H * ((a.Lq + rows - 1) / rows) * a.q_splits;
     const int64_t delta_groups = ((int64_t)a.B * a.H * a.Lp * (s->hd * eb / 16) + kBlock - 1) / kBlock;
     IX_CHECK_ARG(groups < kMostGroups && delta_groups < kMostGroups, "ix_band_attn_bwd: too many rows for one launch");
     a.key_groups = (int)key_groups;
@@ -1157,10 +1204,9 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
 #define BAND_BWD(DT, D) launch_bwd<DT, D>(a, nb, (unsigned)groups, stream)
     BAND_GO(BAND_BWD)
     IX_CHECK_LAUNCH("ix_band_attn_bwd");
-    if (parts) {
-        const int blocks = r.splits > 1 ? r.blocks : r.wide;
-        IX_CHECK_ARG(blocks <= 65535, "ix_band_attn_bwd: too many keys for one launch");
-        const dim3 sgrid(a.B * a.kv, blocks, 4);
+    if (parts || parts_q) {
+        const int k_blocks = r.splits > 1 ? r.blocks : parts ? r.wide : 0, q_blocks = parts_q ? (a.Lq + rows - 1) / rows : 0;   // (both under 65 536)
+        const dim3 sgrid(a.B * (a.kv + (parts_q ? a.H : 0)), k_blocks > q_blocks ? k_blocks : q_blocks, 4);
 #define BAND_SUM(DT, D) band_sum_kernel<DT, D><<<sgrid, kBlock, 0, stream>>>(a, r.items, rows)
         BAND_GO(BAND_SUM)
         IX_CHECK_LAUNCH("ix_band_attn_bwd (sum)");

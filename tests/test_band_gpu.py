@@ -142,6 +142,13 @@ def test_few_queries_over_many_keys(dtype, Lq, Lk, how):
 
 
 @TYPES
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("Lq, Lk, H, kv, how", [(1100, 1100, 1, 1, {}), (400, 2000, 2, 1, dict(window=900, sinks=70)), (90, 1300, 3, 1, dict(causal=False, window=1000))])
+def test_gradients_of_few_rows_in_pieces(dtype, D, Lq, Lk, H, kv, how):
+    check(*inputs(1, Lq, Lk, H, kv, D, dtype), **how)
+
+
+@TYPES
 def test_views(dtype):
     """a packed projection in place, rows off 16 bytes, swapped axes, inputs that are one row many times"""
     from interactron_amd import hipops
