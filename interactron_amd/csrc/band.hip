@@ -988,15 +988,18 @@ int bwd_nb(const ix_band* s) {
     return (int64_t)s->batch * (s->heads * div_up(s->Lq, 128) + s->kv_heads * div_up(s->Lk, 128)) < 600 ? 1 : 2;
 }
 
-// Pieces of the forward's key tiles: where the rows are so few that half of the compute units would stand idle, up to 32 pieces of at least
-// four tiles (40 queries of 16 heads over 6 000 keys: 101 us in one piece).
+// Pieces of the forward's key tiles: where the blocks of queries are fewer than the compute units, about 512 in all, up to 32 of a block and
+// at least four tiles each (eight where more than half of the units have a block: the join costs 4 to 5 us).  One piece / these: bf16, 40
+// queries of 16 heads of 128 over 6 000 keys 101 / 19 us, 6 000 of 2 heads of 64 72 / 35, 3 000 of 4 heads 38 / 24; f32, 6 000 of one head of
+// 128 149 (256 pieces) / 127; fp16, 2 060 of 7 heads of 32 26 / 18.5.  Two pieces of five tiles (3 000 of 4 heads, window 500): 11 / 15.
 int fwd_splits(const ix_band* s) {
     const int64_t groups = (int64_t)s->batch * s->heads * div_up(s->Lq, owner_rows(fwd_nb(s)));
-    if (groups > 128) return 1;
+    if (groups >= 256) return 1;
     const int tb = key_tile(s->dtype);
     const int64_t all = div_up(s->Lk, tb), some = div_up(reach(s) + 64, tb) + 1 + div_up(s->sinks, tb), tiles = some < all ? some : all;
-    int64_t r = 512 / groups;
-    if (r > tiles / 4) r = tiles / 4;
+    const int64_t most = tiles / (groups > 128 ? 8 : 4);
+    int64_t r = div_up(512, groups);
+    if (r > most) r = most;
     return (int)(r < 2 ? 1 : r > 32 ? 32 : r);
 }
 size_t fwd_part(const ix_band* s) {   // partial rows
