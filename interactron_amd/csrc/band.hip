@@ -988,13 +988,15 @@ int bwd_nb(const ix_band* s) {
     return (int64_t)s->batch * (s->heads * div_up(s->Lq, 128) + s->kv_heads * div_up(s->Lk, 128)) < 600 ? 1 : 2;
 }
 
-// Pieces of the forward's key tiles: where the blocks of queries are fewer than the compute units, about 512 in all, up to 32 of a block and
+// Pieces of the forward's key tiles: where the blocks of queries are fewer than two a compute unit, about 512 in all, up to 32 of a block and
 // at least four tiles each (eight where more than half of the units have a block: the join costs 4 to 5 us).  One piece / these: bf16, 40
-// queries of 16 heads of 128 over 6 000 keys 101 / 19 us, 6 000 of 2 heads of 64 72 / 35, 3 000 of 4 heads 38 / 24; f32, 6 000 of one head of
-// 128 149 (256 pieces) / 127; fp16, 2 060 of 7 heads of 32 26 / 18.5.  Two pieces of five tiles (3 000 of 4 heads, window 500): 11 / 15.
+// queries of 16 heads of 128 over 6 000 keys 101 / 19 us, 6 000 of 2 heads of 64 72 / 35, 3 000 of 4 heads 38 / 24, 4 x 512 of 8 heads of 128
+// over 8 192 keys 145 / 115; f32, 4 096 of 4 heads of 64 185 / 145; fp16, 8 192 of 2 heads of 128 136 / 95.  No gain: two pieces of five
+// tiles (3 000 of 4 heads, window 500) 11 / 15, of sixteen (2 060 of 8 heads of 64) 29.5 / 31.  About 768 pieces: 74 us for the 8 192 of 2
+// heads, but 124 for the 4 x 512.
 int fwd_splits(const ix_band* s) {
     const int64_t groups = (int64_t)s->batch * s->heads * div_up(s->Lq, owner_rows(fwd_nb(s)));
-    if (groups >= 256) return 1;
+    if (groups >= 512) return 1;
     const int tb = key_tile(s->dtype);
     const int64_t all = div_up(s->Lk, tb), some = div_up(reach(s) + 64, tb) + 1 + div_up(s->sinks, tb), tiles = some < all ? some : all;
     const int64_t most = tiles / (groups > 128 ? 8 : 4);
@@ -1009,12 +1011,22 @@ size_t fwd_part(const ix_band* s) {   // partial rows
 
 struct KeyPlan { int blocks, wide, wide_splits, splits, items; };
 
+// Pieces of every block in the backward pass, of `wgs` blocks (of keys for dk / dv, of queries for dq) that stream `tiles` tiles of `tb` rows.
+// Fewer blocks than compute units (few heads, or few key heads): about 384 pieces of at least four tiles.  Fewer than two a unit: two pieces of
+// at least 1 536 rows.  Forward and gradients, us: uncut / with 256 / 384 / 512 pieces, f32, 2 x 2 041 of 2 heads of 64 234 / 180 / 146 / 145,
+// 6 000 of one head of 128 977 / 580 / 437 / 453; bf16, 40 queries of 16 heads over 6 000 keys of 4 of 128 159 / 58 / 57 / 68.  256 blocks, one
+// piece / two: 8 192 of 2 heads of 128 429 / 308, 4 096 of 4 heads of 64 in f32 610 / 455, 4 x 512 of 8 heads over 8 192 keys 533 / 461 -- but
+// 2 060 of 8 heads of 64 94 / 100, of 12 heads with window 800 60 / 72.
+int64_t bwd_pieces(int64_t wgs, int64_t tiles, int tb) {
+    int64_t r = wgs < 256 ? div_up(384, wgs) : wgs < 512 ? 2 : 1;
+    const int64_t most = wgs < 256 ? div_up(tiles, 4) : tiles * tb / 1536;
+    if (r > most) r = most;
+    return r < 1 ? 1 : r;
+}
+
 // Splits of dk / dv.  A block of keys streams the queries of its band; a block with some of the first `sinks` keys streams all of them, and
 // where these are more than two and a half times the others' it would run on alone: it is cut into pieces of up to twice the others'
-// length.  Where all blocks together are fewer than the compute units (few key heads, many query heads), every block is cut, into about 384
-// pieces in all: forward and gradients with 256 / 384 / 512 for the keys and for dq, f32, 2 x 2 041 of 2 heads of 64 180 / 146 / 145 us, 6 000 of
-// one head of 128 580 / 437 / 453; bf16, 6 000 of 2 heads of 64 169 / 143 / 142, 40 queries of 16 heads over 6 000 keys of 4 of 128 58 / 57 / 68.
-// With 264 blocks (2 060 of 8 heads, every key) two pieces each cost 5 us more than none.
+// length.
 KeyPlan key_plan(const ix_band* s) {
     KeyPlan r;
     const int rows = owner_rows(bwd_nb(s)), group = s->heads / s->kv_heads, tb = query_tile(s->dtype, s->hd);
@@ -1022,9 +1034,7 @@ KeyPlan key_plan(const ix_band* s) {
     r.wide = s->sinks > 0 ? (s->sinks < s->Lk ? (int)div_up(s->sinks, rows) : r.blocks) : 0;
     const int64_t all = div_up(s->Lq, tb), band = div_up(reach(s) + rows, tb) + 1, each = (band < all ? band : all) * group;
     const int64_t wgs = (int64_t)s->batch * s->kv_heads * r.blocks;
-    int64_t sp = wgs < 256 ? div_up(384, wgs) : 1;
-    if (sp > div_up(each, 4)) sp = div_up(each, 4);   // (no piece under four tiles)
-    r.splits = (int)(sp < 1 ? 1 : sp);
+    r.splits = (int)bwd_pieces(wgs, each, tb);
     const int64_t piece = div_up(each, r.splits);
     int64_t ws = 2 * all * group <= 5 * piece ? 1 : div_up(all * group, 2 * piece);
     const int64_t wide = (int64_t)s->batch * s->kv_heads * r.wide;
@@ -1035,16 +1045,11 @@ KeyPlan key_plan(const ix_band* s) {
     return r;
 }
 
-// Pieces of dq's key tiles, by the same rule as the keys' blocks: at least four tiles each, where the blocks of queries are fewer than the
-// compute units (uncut: 40 queries of 16 heads over 6 000 keys 159 us instead of 58, 6 000 of one head of 128 in f32 977 instead of 580).
 int dq_splits(const ix_band* s) {
-    const int64_t groups = (int64_t)s->batch * s->heads * div_up(s->Lq, owner_rows(bwd_nb(s)));
-    if (groups >= 256) return 1;
-    const int tb = key_tile(s->dtype);
-    const int64_t all = div_up(s->Lk, tb), some = div_up(reach(s) + owner_rows(bwd_nb(s)), tb) + 1 + div_up(s->sinks, tb), tiles = some < all ? some : all;
-    int64_t r = div_up(384, groups);
-    if (r > tiles / 4) r = tiles / 4;
-    return (int)(r < 2 ? 1 : r > 32 ? 32 : r);
+    const int rows = owner_rows(bwd_nb(s)), tb = key_tile(s->dtype);
+    const int64_t all = div_up(s->Lk, tb), some = div_up(reach(s) + rows, tb) + 1 + div_up(s->sinks, tb);
+    const int64_t r = bwd_pieces((int64_t)s->batch * s->heads * div_up(s->Lq, rows), some < all ? some : all, tb);
+    return (int)(r > 32 ? 32 : r);
 }
 size_t dq_part_bytes(const ix_band* s) {
     const int r = dq_splits(s), rows = owner_rows(bwd_nb(s));
