@@ -99,10 +99,12 @@ class PagedCache:
         if table.dim() != 2 or not table.numel() or not total or not kv:
             raise ValueError("an empty cache, or a page table that is not [batch, pages]: %s, %s" % (list(shape), list(table.shape)))
         B, pages = table.shape
-        _whole(k, "cache keys", dtype, shape)
-        _whole(v, "cache values", dtype, shape)
-        _whole(table, "the page table", torch.int32, (B, pages))
-        _whole(lens, "the lengths", torch.int32, (B,))
+        if not (v.shape == shape and v.dtype is dtype and table.dtype is torch.int32 and lens.dtype is torch.int32 and lens.shape == (B,) and
+                k.is_contiguous() and v.is_contiguous() and table.is_contiguous() and lens.is_contiguous()):
+            _whole(k, "cache keys", dtype, shape)   # (says which)
+            _whole(v, "cache values", dtype, shape)
+            _whole(table, "the page table", torch.int32, (B, pages))
+            _whole(lens, "the lengths", torch.int32, (B,))
         if weight is not None:
             _whole(weight, "the weights", torch.float32, (B, kv, pages * page))
         if B > 65535 or kv > 1024 or pages * page >= 1 << 30 or total >= 1 << 31:
