@@ -237,6 +237,18 @@ def test_inputs_changed_in_between_are_noticed():
 
 
 @TYPES
+def test_a_graph_kept_for_two_backward_passes(dtype):
+    from interactron_amd import hipops
+    q, k, v, do = inputs(1, 500, 500, 4, 2, 64, dtype)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = hipops.band_attention(*leaves, sinks=2)
+    out.backward(do, retain_graph=True)
+    once = [t.grad.clone() for t in leaves]
+    out.backward(do)
+    assert all(torch.equal(t.grad, 2 * g) for t, g in zip(leaves, once))
+
+
+@TYPES
 def test_saved_tensors_kept_elsewhere(dtype):
     """hooks that move what the forward pass saves: the gradients come from the tensors that come back"""
     from interactron_amd import hipops
@@ -267,14 +279,16 @@ def test_the_same_call_gives_the_same_bits(D):
         assert all(torch.equal(a, b) for a, b in zip(first, once()))
 
 
-def test_captured_and_replayed_with_gradients():
+@pytest.mark.parametrize("L", [300, 900])
+def test_captured_and_replayed_with_gradients(L):
+    """(900: all three gradients and the output in pieces)"""
     from interactron_amd import hipops
-    q, k, v, do = inputs(2, 300, 300, 4, 2, 64, BF16)
-    n = torch.tensor([300, 200], dtype=torch.int32, device="cuda")
+    q, k, v, do = inputs(2, L, L, 4, 2, 64, BF16)
+    n = torch.tensor([L, L - 100], dtype=torch.int32, device="cuda")
 
     def step():
         t = [x.detach().requires_grad_(True) for x in (q, k, v)]
-        out = hipops.band_attention(*t, window=70, sinks=5, q_lens=n, kv_lens=n)
+        out = hipops.band_attention(*t, window=70 if L == 300 else None, sinks=5, q_lens=n, kv_lens=n)
         return (out.detach(),) + torch.autograd.grad(out, t, do)
 
     side = torch.cuda.Stream()
@@ -289,7 +303,7 @@ def test_captured_and_replayed_with_gradients():
     for i in range(6):
         for t in (q, k, v, do):
             t.copy_(torch.randn(t.shape, generator=g).to(BF16))
-        n.copy_(torch.tensor([300 - 20 * i, 10 * i], dtype=torch.int32))
+        n.copy_(torch.tensor([L - 20 * i, 10 * i], dtype=torch.int32))
         graph.replay()
         want = step()
         torch.cuda.synchronize()
