@@ -975,13 +975,15 @@ int64_t reach(const ix_band* s) {   // rows on both sides that a band takes from
 }
 
 // Owner rows: 64 or 128 a workgroup (one or two blocks of 16 for every wave).  Two blocks read LDS half as often for the same products, one
-// gives twice as many workgroups and waves.  Measured, bf16 (us, one / two): forward head dim 64, 64 workgroups of 128 rows 9 / 13, 272 of
-// them 24 / 28, 800 of them 120 / 105; head dim 32, 544: 27 / 30, 1 024: 142 / 132; head dim 128, where LDS counts double, 64: 14 / 18,
-// 512: 66 / 57, 2 048: 399 / 310.  Gradients head dim 64, 192: 12.6 / 15, 576: 49 / 49, 1 632: 322 / 284; head dim 128 only one (two take
-// the registers of a second wave: 20 / 37 at 176, 667 / 913 at 2 048).  f32 has room for one.
+// gives twice as many workgroups and waves, and evens out the lengths of causal rows.  Measured, bf16 (us, one / two, by the number of
+// workgroups of 128 rows): forward head dim 64, 64: 9 / 13, 272: 24 / 28, 800: 120 / 105; head dim 32, 544: 27 / 30, 1 024: 142 / 132; head dim
+// 128, where LDS counts double, 64: 14 / 18, 256: 25 / 31 causal and 30 / 32 not, 384: 40 / 46 causal but 68 / 60 not and 28 / 25 with a window,
+// 448: 48 / 50, 85 / 69 and 48 / 42, 512: 66 / 57, 2 048: 399 / 310.  Gradients head dim 64, 192: 12.6 / 15, 576: 49 / 49, 1 632: 322 / 284; head
+// dim 128 only one (two take the registers of a second wave: 20 / 37 at 176, 667 / 913 at 2 048).  f32 has room for one.
 int fwd_nb(const ix_band* s) {
     if (s->dtype == 0) return 1;
-    return (int64_t)s->batch * s->heads * div_up(s->Lq, 128) < (s->hd == 128 ? 256 : 600) ? 1 : 2;
+    const int few = s->hd < 128 ? 600 : s->causal && s->window == 0 ? 512 : 384;
+    return (int64_t)s->batch * s->heads * div_up(s->Lq, 128) < few ? 1 : 2;
 }
 int bwd_nb(const ix_band* s) {
     if (s->dtype == 0 || s->hd == 128) return 1;
@@ -993,10 +995,11 @@ int bwd_nb(const ix_band* s) {
 // queries of 16 heads of 128 over 6 000 keys 101 / 19 us, 6 000 of 2 heads of 64 72 / 35, 3 000 of 4 heads 38 / 24, 4 x 512 of 8 heads of 128
 // over 8 192 keys 145 / 115; f32, 4 096 of 4 heads of 64 185 / 145; fp16, 8 192 of 2 heads of 128 136 / 95.  No gain: two pieces of five
 // tiles (3 000 of 4 heads, window 500) 11 / 15, of sixteen (2 060 of 8 heads of 64) 29.5 / 31.  About 768 pieces: 74 us for the 8 192 of 2
-// heads, but 124 for the 4 x 512.
+// heads, but 124 for the 4 x 512.  Blocks of 128 rows, of which a compute unit holds half as many, stay whole (384 of them with 1 536 keys of hd
+// 128 46 / 58, 448 with window 512 42 / 65).
 int fwd_splits(const ix_band* s) {
     const int64_t groups = (int64_t)s->batch * s->heads * div_up(s->Lq, owner_rows(fwd_nb(s)));
-    if (groups >= 512) return 1;
+    if (groups >= 512 || fwd_nb(s) == 2) return 1;
     const int tb = key_tile(s->dtype);
     const int64_t all = div_up(s->Lk, tb), some = div_up(reach(s) + 64, tb) + 1 + div_up(s->sinks, tb), tiles = some < all ? some : all;
     const int64_t most = tiles / (groups > 128 ? 8 : 4);
