@@ -288,15 +288,17 @@ template <int DT> __device__ __forceinline__ Frag<DT> as_frag(const f32x4& a, co
     return f;
 }
 
-// ... and the operand of what that rounding took away.  Score gradients go into dq and dk as these two terms: with one, the error of dq and
-// dk against 64 bits is 1.45 to 1.7 times that of their own rounding, with two 1.0 times; it costs 60 of 335 us (bf16, 12 755 queries and
-// keys of 8 heads of 64, window 2 551).  Weights go into the outputs and dv as one term (1.4 times; two would cost 33 of 105 us).
+// ... and the operand of what that rounding took away.  Weights (into the outputs and dv) and score gradients (into dq and dk) are carried as
+// these two terms: outputs and gradients are then as good as from 32-bit ones.  With one term the error against 64 bits is 1.4 (outputs, dv)
+// and 1.45 to 1.7 times (dq, dk) that of the result's own rounding, with two 1.0 times.  The second terms of the weights cost 58 of 446 us
+// (forward and gradients, bf16, 12 755 queries and keys of 8 heads of 64, window 2 551) and 67 of 347 us (forward, fp16, 8 192 of 32 heads
+// over 8 of 128, window 2 048), those of the score gradients 60 us of the former.
 template <int DT> __device__ __forceinline__ Frag<DT> rest_frag(const f32x4& a, const f32x4& b, const Frag<DT>& f) {
     Frag<DT> r;
-    r.w[0] = seq_pack<DT>(a[0] - seq_lo<DT>(f.w[0]), a[1] - seq_hi<DT>(f.w[0]));
-    r.w[1] = seq_pack<DT>(a[2] - seq_lo<DT>(f.w[1]), a[3] - seq_hi<DT>(f.w[1]));
-    r.w[2] = seq_pack<DT>(b[0] - seq_lo<DT>(f.w[2]), b[1] - seq_hi<DT>(f.w[2]));
-    r.w[3] = seq_pack<DT>(b[2] - seq_lo<DT>(f.w[3]), b[3] - seq_hi<DT>(f.w[3]));
+    r.w[0] = seq_pack<DT>(seq_less_lo<DT>(a[0], f.w[0]), seq_less_hi<DT>(a[1], f.w[0]));
+    r.w[1] = seq_pack<DT>(seq_less_lo<DT>(a[2], f.w[1]), seq_less_hi<DT>(a[3], f.w[1]));
+    r.w[2] = seq_pack<DT>(seq_less_lo<DT>(b[0], f.w[2]), seq_less_hi<DT>(b[1], f.w[2]));
+    r.w[3] = seq_pack<DT>(seq_less_lo<DT>(b[2], f.w[3]), seq_less_hi<DT>(b[3], f.w[3]));
     return r;
 }
 
@@ -344,8 +346,7 @@ constexpr float kFirstF = 1099511627776.f;   // 2^40
 // forward
 // ====================================================================================================================================
 // The running maximum is raised only where a tile exceeds it by more than 2^8 (a weight may then reach 256, exact in all types' ranges):
-// most tiles leave the accumulators alone.  16-bit types: a weight is rounded once to the type for the second product (half a step, like
-// the result itself: against 64 bits the two add up to sqrt(2) times the result's own rounding); the sum takes the unrounded weights.
+// most tiles leave the accumulators alone.  16-bit types: a weight goes into the second product as two terms (rest_frag), into the sum unrounded.
 // Bound by matrix and vector instructions together (matrix pipe 43 % and vector instructions 51 % of busy cycles at hd 128, 33 and 63 % at
 // hd 64, a tenth of the time for the bytes, no LDS conflicts): fp16, 8 192 queries and keys of 32 / 8 heads of 128, window 2 048: 275 us =
 // 875 TFLOP/s, 0.75 of what a plain product of 8 192^3 reaches; bf16, 12 755 of 8 heads of 64, window 2 551: 89-103 us = 580-680 TFLOP/s (a
@@ -456,11 +457,15 @@ __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) 
                 constexpr int KK = SB / 2, TOGETHER = I::DB == 8 ? 1 : KK;
 #pragma unroll
                 for (int k0 = 0; k0 < KK; k0 += TOGETHER) {
-                    Frag<DT> pf[TOGETHER][NB];
+                    Frag<DT> pf[TOGETHER][NB], pr[TOGETHER][NB];
 #pragma unroll
                     for (int kk = 0; kk < TOGETHER; ++kk)
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) pf[kk][nb] = as_frag<DT>(s[nb][2 * (k0 + kk)], s[nb][2 * (k0 + kk) + 1]);
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const f32x4 &x = s[nb][2 * (k0 + kk)], &y = s[nb][2 * (k0 + kk) + 1];
+                            pf[kk][nb] = as_frag<DT>(x, y);
+                            if constexpr (DT != 0) pr[kk][nb] = rest_frag<DT>(x, y, pf[kk][nb]);
+                        }
 #pragma unroll
                     for (int d0 = 0; d0 < I::DB; d0 += I::DN) {
                         Frag<DT> vf[TOGETHER][I::DN];
@@ -470,7 +475,10 @@ __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) 
 #pragma unroll
                             for (int db = 0; db < I::DN; ++db)
 #pragma unroll
-                                for (int nb = 0; nb < NB; ++nb) o[nb][d0 + db] = seq_mma<DT>(vf[kk][db], pf[kk][nb], o[nb][d0 + db]);
+                                for (int nb = 0; nb < NB; ++nb) {
+                                    if constexpr (DT != 0) o[nb][d0 + db] = seq_mma<DT>(vf[kk][db], pr[kk][nb], o[nb][d0 + db]);
+                                    o[nb][d0 + db] = seq_mma<DT>(vf[kk][db], pf[kk][nb], o[nb][d0 + db]);
+                                }
                     }
                 }
             }
@@ -847,7 +855,7 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
                                 for (int e = 0; e < 4; ++e) s[nb][x][e] = r.in(p0 + 4 * g + 32 * kk + 16 * x + e) ? s[nb][x][e] : 0.f;
                         }
                     }
-                    Frag<DT> pf[NB], zf[NB], zr[NB];
+                    Frag<DT> pf[NB], pr[NB], zf[NB], zr[NB];
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -868,7 +876,10 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
                         }
                         pf[nb] = as_frag<DT>(s[nb][0], s[nb][1]);
                         zf[nb] = as_frag<DT>(z[nb][0], z[nb][1]);
-                        if constexpr (DT != 0) zr[nb] = rest_frag<DT>(z[nb][0], z[nb][1], zf[nb]);
+                        if constexpr (DT != 0) {
+                            pr[nb] = rest_frag<DT>(s[nb][0], s[nb][1], pf[nb]);
+                            zr[nb] = rest_frag<DT>(z[nb][0], z[nb][1], zf[nb]);
+                        }
                     }
 #pragma unroll
                     for (int d0 = 0; d0 < I::DB; d0 += I::DN) {
@@ -878,6 +889,7 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
                         for (int db = 0; db < I::DN; ++db)
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
+                                if constexpr (DT != 0) av[nb][d0 + db] = seq_mma<DT>(gq[0][db], pr[nb], av[nb][d0 + db]);
                                 av[nb][d0 + db] = seq_mma<DT>(gq[0][db], pf[nb], av[nb][d0 + db]);
                                 if constexpr (DT != 0) ak[nb][d0 + db] = seq_mma<DT>(gq[1][db], zr[nb], ak[nb][d0 + db]);
                                 ak[nb][d0 + db] = seq_mma<DT>(gq[1][db], zf[nb], ak[nb][d0 + db]);
@@ -914,7 +926,7 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
 }
 
 // Both in one launch, the key blocks first: either alone would leave compute units empty at the sizes where time counts, and at its end.
-// Nine products of 2 hd operations a pair (four of the formulas, q k^T and do v^T twice, the second terms of dz): 12 755 queries and keys of 8
+// Ten products of 2 hd operations a pair (four of the formulas, q k^T and do v^T twice, the second terms of P and dz): 12 755 queries and keys of 8
 // heads of 64, window 2 551, bf16: 307-343 us = 790-900 TFLOP/s, matrix pipe 43 % and vector instructions 56 % of busy cycles; head dim 128 at
 // 8 192 of 32 / 8 heads, window 2 048: 1 317 us = 820 TFLOP/s; f32, 16 x 361 of 8 heads of 32, window 64: 47 us.  Scores of the next 32 rows
 // ahead of this one's exponentials: 350 / 350 us.

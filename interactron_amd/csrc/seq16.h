@@ -52,6 +52,29 @@ template <int DT> __device__ __forceinline__ float seq_hi(unsigned w) {
     if constexpr (DT == 1) return __uint_as_float(w & 0xffff0000u);
     else return (float)__builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
 }
+// x less the lower / upper of two 16-bit values.  fp16: one v_fma_mix_f32 that reads the half where it is (written as a conversion and a
+// difference the compiler rounds x a second time instead of taking the half out of its register).  x must not be a matrix instruction's own
+// result: the compiler puts no wait for that before the instruction.
+template <int DT> __device__ __forceinline__ float seq_less_lo(float x, unsigned w) {
+    if constexpr (DT == 1) return x - seq_lo<DT>(w);
+#ifdef __HIP_DEVICE_COMPILE__
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(x));
+    return r;
+#else
+    return x - seq_lo<DT>(w);
+#endif
+}
+template <int DT> __device__ __forceinline__ float seq_less_hi(float x, unsigned w) {
+    if constexpr (DT == 1) return x - seq_hi<DT>(w);
+#ifdef __HIP_DEVICE_COMPILE__
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(x));
+    return r;
+#else
+    return x - seq_hi<DT>(w);
+#endif
+}
 template <int DT> __device__ __forceinline__ void seq_store1(void* p, int64_t i, float x) {
     if constexpr (DT == 0) static_cast<float*>(p)[i] = x;
     else static_cast<unsigned short*>(p)[i] = (unsigned short)(seq_pack<DT>(x, 0.f) & 0xffffu);

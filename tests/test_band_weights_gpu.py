@@ -1,0 +1,25 @@
+"""The softmax weights of band attention in its products with v and do (tests/band_bounds.py)."""
+import pytest
+import torch
+
+from tests import band_bounds as bounds
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def inputs(B, Lq, Lk, H, kv, D, dtype, seed=0, scale=1.5):
+    g = torch.Generator().manual_seed(seed)
+    make = lambda L, h, s=1.0: (torch.randn(B, L, h, D, generator=g) * s).to(dtype).cuda()  # noqa: E731
+    return make(Lq, H, scale), make(Lk, kv), make(Lk, kv), make(Lq, H)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("Lq, Lk, how", [(200, 200, dict(window=60, sinks=3)), (200, 200, dict(causal=False)), (5, 1500, {}), (700, 700, dict(sinks=70, window=30))],
+                         ids=["band", "full", "pieces", "first keys"])
+def test_weights_are_as_good_as_32_bit_ones(dtype, D, Lq, Lk, how):
+    """out and dv are off by their own rounding and what 32-bit arithmetic leaves, not by a rounding of the weights"""
+    # (fp16: steps below 2^-14 are 2^-24, half of one off; a row's largest weight is 1 in the forward pass)
+    bounds.check(*inputs(2, Lq, Lk, 4, 2, D, dtype, seed=D), floor=2.0 ** -25 if dtype is FP16 else 0.0, **how)
