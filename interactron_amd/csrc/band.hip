@@ -352,6 +352,12 @@ constexpr float kFirstF = 1099511627776.f;   // 2^40
 // 875 TFLOP/s, 0.75 of what a plain product of 8 192^3 reaches; bf16, 12 755 of 8 heads of 64, window 2 551: 89-103 us = 580-680 TFLOP/s (a
 // score costs as much exponential for half the product); 2 060 of 16 heads of 64, window 412: 24 us, its 528 workgroups' first and last tiles.
 constexpr float kSlack = 8.f;
+// fp16: weights are carried 2^7 and, for dv, 2^12 times as large (the largest forward weight, 2^8 by the slack, is then 2^15; the type ends at
+// 65 504), so that its smallest step, 2^-24, is 2^-31 of the row's largest weight and 2^-36: a row whose first key takes nearly all the weight
+// keeps what the others have.
+template <int DT> constexpr float kUp = DT == 2 ? 7.f : 0.f;
+template <int DT> constexpr float kUpFactor = DT == 2 ? 128.f : 1.f;
+template <int DT> constexpr float kUpDv = DT == 2 ? 4096.f : 1.f;
 
 template <int DT, int D, int NB, int TB>
 __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) {
@@ -444,7 +450,7 @@ __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) 
 #pragma unroll
                         for (int db = 0; db < I::DB; ++db) o[nb][db] *= down;
                     }
-                    const float ref = top[nb] == -INFINITY ? 0.f : top[nb];
+                    const float ref = (top[nb] == -INFINITY ? 0.f : top[nb]) - kUp<DT>;
 #pragma unroll
                     for (int sb = 0; sb < SB; ++sb)
 #pragma unroll
@@ -491,14 +497,14 @@ __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) 
         if (a.fwd_splits > 1) {   // what this piece has, for band_join_kernel
             if (i >= a.Lq) continue;
             const int64_t at = ((int64_t)bh * a.Lq + i) * a.fwd_splits + blockIdx.z;
-            if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{top[nb], total};
+            if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{top[nb], total / kUpFactor<DT>};
 #pragma unroll
-            for (int db = 0; db < I::DB; ++db) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * db + 4 * g) = o[nb][db];
+            for (int db = 0; db < I::DB; ++db) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * db + 4 * g) = o[nb][db] * (1.f / kUpFactor<DT>);
             continue;
         }
         const bool none = i >= m || total == 0.f;
         const float inv = 1.f / total;
-        if (a.lse && g == 0 && i < a.Lp) a.lse[(int64_t)bh * a.Lp + i] = none ? INFINITY : top[nb] + __log2f(total);
+        if (a.lse && g == 0 && i < a.Lp) a.lse[(int64_t)bh * a.Lp + i] = none ? INFINITY : top[nb] - kUp<DT> + __log2f(total);
         if (i >= a.Lq) continue;
         const int64_t at = (((int64_t)b * a.Lq + i) * a.H + h) * I::ROW;
 #pragma unroll
@@ -871,8 +877,8 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
                             fit16<I::DB>(mx, F[nb], ak[nb]);
                             z[nb][0] *= F[nb];
                             z[nb][1] *= F[nb];
-                            s[nb][0] *= 1024.f;   // (weights of long rows stay clear of the type's smallest steps)
-                            s[nb][1] *= 1024.f;
+                            s[nb][0] *= kUpDv<DT>;
+                            s[nb][1] *= kUpDv<DT>;
                         }
                         pf[nb] = as_frag<DT>(s[nb][0], s[nb][1]);
                         zf[nb] = as_frag<DT>(z[nb][0], z[nb][1]);
@@ -902,7 +908,7 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const int row = wave * 16 * NB + 16 * nb + n16, j = j0 + row;
-        const float fk = DT == 2 ? a.scale / F[nb] : a.scale, fv = DT == 2 ? 1.f / 1024.f : 1.f;
+        const float fk = DT == 2 ? a.scale / F[nb] : a.scale, fv = 1.f / kUpDv<DT>;
         if (j >= n) {   // (padding: columns beside the valid ones of this block)
 #pragma unroll
             for (int db = 0; db < I::DB; ++db) ak[nb][db] = av[nb][db] = f32x4{0.f, 0.f, 0.f, 0.f};

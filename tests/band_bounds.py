@@ -17,10 +17,10 @@ def close(got, want, err, name=""):
     assert (off <= tol).all(), (name, float((off / tol).max()), np.unravel_index((off / tol).argmax(), off.shape), int((off > tol).sum()), off.size)
 
 
-def band(q, k, v, window=None, sinks=0, causal=True, scale=None, q_lens=None, kv_lens=None, do=None, floor=0.0):
+def band(q, k, v, window=None, sinks=0, causal=True, scale=None, q_lens=None, kv_lens=None, do=None, floor=0.0, floor_dv=None):
     """-> values and errors as sequence_reference.band_attention gives them, the errors of out and dv with weights as two terms of the
     type.  h: half a step; a term leaves h of what it rounds, two leave h^2 (2 h^2 allowed).  floor: the smallest step of the second
-    term, absolute, as a share of the row's largest weight (fp16)."""
+    term, absolute, as a share of the row's largest weight; floor_dv (default: the same): the same of a weight in dv (fp16)."""
     lens = {x: t.cpu() for x, t in (("q_lens", q_lens), ("kv_lens", kv_lens)) if t is not None}
     val, err = ref.band_attention(q, k, v, window, sinks, causal, scale, do=do, **lens)
     two = 0.0 if q.dtype == torch.float32 else 2 * ref.half_step(q.dtype) ** 2
@@ -42,14 +42,14 @@ def band(q, k, v, window=None, sinks=0, causal=True, scale=None, q_lens=None, kv
             rel = 2 * (D + 8) * ref.U * worst + (n / 16 + 64) * ref.U
             err["out"][b, :m, i] = (p * (rel + two) + floor * see * p.max(1, keepdims=True)) @ np.abs(vv)
             if do is not None:
-                err["dv"][b, :n, i // G] += (p * (rel + two + (m / 16 + 64 + 8 * G) * ref.U) + floor * see).T @ np.abs(do[b, :m, i])
+                err["dv"][b, :n, i // G] += (p * (rel + two + (m / 16 + 64 + 8 * G) * ref.U) + (floor if floor_dv is None else floor_dv) * see).T @ np.abs(do[b, :m, i])
     return val, err
 
 
-def check(q, k, v, do=None, floor=0.0, **how):
+def check(q, k, v, do=None, floor=0.0, floor_dv=None, **how):
     """the call against the bounds above"""
     from interactron_amd import hipops
-    want, err = band(q, k, v, do=do, floor=floor, **how)
+    want, err = band(q, k, v, do=do, floor=floor, floor_dv=floor_dv, **how)
     if do is None:
         out = hipops.band_attention(q, k, v, **how)
         close(out, want["out"], err["out"], "out")

@@ -23,3 +23,23 @@ def test_weights_are_as_good_as_32_bit_ones(dtype, D, Lq, Lk, how):
     """out and dv are off by their own rounding and what 32-bit arithmetic leaves, not by a rounding of the weights"""
     # (fp16: steps below 2^-14 are 2^-24, half of one off; a row's largest weight is 1 in the forward pass)
     bounds.check(*inputs(2, Lq, Lk, 4, 2, D, dtype, seed=D), floor=2.0 ** -25 if dtype is FP16 else 0.0, **how)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("Lq, Lk, how", [(200, 200, dict(window=60, sinks=3)), (300, 300, dict(window=40, sinks=1)), (7, 2000, dict(window=90, sinks=1))], ids=["band", "first key", "pieces"])
+@pytest.mark.parametrize("lead", [0.0, 12.0, 17.0, 24.0])
+def test_small_weights_in_fp16(D, Lq, Lk, how, lead):
+    """the first key stands `lead` above the others and its value is zero: outputs and dv are made of the small weights alone.  Half the type's
+    smallest step, 2^-25, is 2^-32 of the row's largest weight (carried 2^7 times as large, or more), and 2^-37 in dv (2^12 times)"""
+    q, k, v, do = inputs(2, Lq, Lk, 4, 2, D, FP16, seed=int(lead), scale=0.5)
+    if lead:
+        q[..., 0], k[..., 0] = 4.0, 0.0
+        k[:, 0] = 0.0
+        k[:, 0, :, 0] = lead * D ** 0.5 / 4
+        v *= 1e4
+        v[:, 0] = 0.0
+        do *= 1e4
+    bounds.check(q, k, v, None, floor=2.0 ** -32, **how)
+    # (gradients: values and do that keep do v within the type's range)
+    got = bounds.check(q, k, v * 1e-4, do * 1e-2, floor=2.0 ** -32, floor_dv=2.0 ** -37, **how)
+    assert lead == 0 or float(got["dv"][:, 1:].abs().max()) > 0
