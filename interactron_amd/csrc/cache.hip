@@ -104,6 +104,7 @@ struct AttnArgs {
 };
 
 template <int DT> constexpr int tile_keys() { return DT == 0 ? 16 : 32; }
+template <int DT> constexpr float up_exponent() { return DT == 2 ? 15.f : 0.f; }
 
 template <int N> __device__ __forceinline__ void load_words(unsigned* w, const unsigned char* p) {
     if constexpr (N >= 4) {
@@ -127,7 +128,8 @@ template <int N> __device__ __forceinline__ void load_words(unsigned* w, const u
 //   the keys 4 g + r (and 16 + 4 g + r): a wave reads whole rows, and with 16-bit values one v_perm_b32 per register turns two rows
 //   into the pairs of keys that the matrix instruction wants.  P comes out of the scores' accumulator in exactly that key order.
 // P is carried as two 16-bit terms (hi + the rest), so that the sum keeps the precision of the f32 weights: the launch is bound by the
-// bytes of K and V, the second matrix instruction is free.
+// bytes of K and V, the second matrix instruction is free.  fp16: carried 2^15 times as large, so that the type's smallest step, 2^-24, is 2^-39
+// of the largest weight and not a share of what a row has besides one dominant key.
 // bf16, 32 heads over 8 of 128: one sequence of 131 071 tokens (537 MB) 94 us = 5.7 TB/s, 32 of 700 to 8 192 (583 MB) 111 us = 5.3 TB/s, where
 // a kernel that only reads reaches 6.2; 411 tokens of 8 heads in f32: 8.8 us, the chain length -> page -> rows -> join in a launch.
 template <int DT, int D, int WAVES>
@@ -232,9 +234,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_kernel(AttnArgs p) {
         const float mn = fmaxf(m, seq_max_g(top)), ref = mn == -INFINITY ? 0.f : mn, alpha = seq_exp2(m - ref);
         float sum = 0.f;
         float pr[VK];
+        const float low = ref - up_exponent<DT>();
 #pragma unroll
         for (int i = 0; i < VK; ++i) {
-            pr[i] = seq_exp2(x[i / 4][i % 4] - ref);
+            pr[i] = seq_exp2(x[i / 4][i % 4] - low);
             sum += pr[i];
         }
         m = mn;
@@ -284,6 +287,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_kernel(AttnArgs p) {
             acc += f * lds_o[w][q][d];
         }
         const int64_t at = (int64_t)b * p.heads + head0 + q;
+        if (DT == 2) {
+            acc *= 1.f / 32768.f;
+            sum *= 1.f / 32768.f;
+        }
         if (p.part_ml) {
             p.part_o[(at * p.splits + split) * D + d] = acc;
             if (d == 0) { p.part_ml[(at * p.splits + split) * 2] = top; p.part_ml[(at * p.splits + split) * 2 + 1] = sum; }
