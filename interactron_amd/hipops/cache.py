@@ -31,6 +31,9 @@ class _CacheC(ctypes.Structure):   # struct ix_paged_cache of include/interactro
 
 
 _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+# for tensors that a kernel has written: a graph that saved one of them raises at its backward pass, as it does after torch's own in-place
+# operations, instead of computing with the new values  (the accessor without the wrapper's checks is 1 us cheaper)
+_written = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
 
 
 def _here(names, *ts):
@@ -76,9 +79,10 @@ class PagedCache:
     lens     int32 [batch]: tokens held
     weight   float32 [batch, kv_heads, pages * page] or None: the attention each token has had so far
     The tensors are written in place, so none of them may require a gradient, and they cannot be exchanged for others (make another cache:
-    it costs nothing but the checks).
+    it costs nothing but the checks).  A call that writes some of them raises their version counters: a graph that saved one (the lengths of
+    band_attention, say) refuses its backward pass afterwards.  (The replay of a captured call does not, like that of torch's own.)
     """
-    __slots__ = ("_k", "_v", "_table", "_lens", "_weight", "kv_heads", "hd", "page", "batch", "pages", "capacity", "dtype", "c", "ref")
+    __slots__ = ("_k", "_v", "_table", "_lens", "_weight", "kv_heads", "hd", "page", "batch", "pages", "capacity", "dtype", "c", "ref", "_all")
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
@@ -121,6 +125,7 @@ class PagedCache:
         self.kv_heads, self.hd, self.page, self.batch, self.pages, self.capacity = kv, hd, page, B, pages, pages * page
         self.c = _CacheC(pk, pv, table.data_ptr(), lens.data_ptr(), None if weight is None else weight.data_ptr(), total, code, kv, page, hd, B, pages)
         self.ref = ctypes.byref(self.c)
+        self._all = (k, v, lens) if weight is None else (k, v, lens, weight)   # what cache_append and cache_compact write
 
 
 def _rows(t, name, cache, shape):
@@ -159,6 +164,7 @@ def cache_append(cache, k, v, counts=None, at=None):
     rc = _L().ix_cache_append(cache.ref, k.data_ptr(), v.data_ptr(), T, kb, kt, kh, vb, vt, vh, n, start, s)
     if rc:
         _chk(rc, "ix_cache_append")
+    _written(cache._all)
 
 
 _attn_ws_bytes = {}   # workspace of ix_cache_attn by sizes
@@ -205,6 +211,8 @@ def cache_attention(q, cache, scale=None, window=None, sinks=0, accumulate=False
     rc = _L().ix_cache_attn(cache.ref, q.data_ptr(), qb, qh, out.data_ptr(), H, scale, w, sinks, accumulate, None if ws is None else ws.data_ptr(), need, s)
     if rc:
         _chk(rc, "ix_cache_attn")
+    if accumulate:
+        _written((cache._weight,))
     return out
 
 
@@ -244,6 +252,7 @@ def cache_compact(cache, kept, left):
         raise ValueError("left must not be the cache's own lengths")
     s = _here(("kept", "left"), kept, left)
     _chk(_L().ix_cache_compact(cache.ref, kept.data_ptr(), left.data_ptr(), kept.shape[2], s), "ix_cache_compact")
+    _written(cache._all)
 
 
 def cache_evict(cache, budget, sinks=0, recent=0):
