@@ -16,7 +16,7 @@ import torch
 
 from .. import _lib
 from . import core
-from .core import _L, _chk, _stream
+from .core import _L, _chk, _no_tangents, _stream
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _HEAD_DIMS = (32, 64, 128)
@@ -115,6 +115,7 @@ class PagedCache:
             raise ValueError("a cache of %d sequences, %d key heads, %d tokens a sequence is too large" % (B, kv, pages * page))
         if k.requires_grad or v.requires_grad or (weight is not None and weight.requires_grad):
             raise _lib.HipLibraryError("the tensors of a cache are written in place: none of them may require a gradient")
+        _no_tangents("a paged cache", (k, v, weight))
         dev, at = core._dev[0], k.get_device()
         if at != dev or v.get_device() != at or table.get_device() != at or lens.get_device() != at or (weight is not None and weight.get_device() != at):
             _here(_CACHE_NAMES, k, v, table, lens, weight)   # (says which; or binds the device at the first call)
@@ -160,6 +161,7 @@ def cache_append(cache, k, v, counts=None, at=None):
     n, start = _per_sequence(counts, "counts", cache), _per_sequence(at, "at", cache)
     if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise _lib.HipLibraryError("cache_append has no backward: call it under torch.no_grad()")
+    _no_tangents("cache_append", (k, v))
     s = _here(("new keys", "new values", "counts", "at"), k, v, counts, at)
     rc = _L().ix_cache_append(cache.ref, k.data_ptr(), v.data_ptr(), T, kb, kt, kh, vb, vt, vh, n, start, s)
     if rc:
@@ -197,6 +199,7 @@ def cache_attention(q, cache, scale=None, window=None, sinks=0, accumulate=False
     shape = (cache.batch, H, cache.hd)
     if q.requires_grad and torch.is_grad_enabled():
         raise _lib.HipLibraryError("cache_attention has no backward: call it under torch.no_grad()")
+    _no_tangents("cache_attention", (q,))
     q, (qb, qh, _) = _rows(q, "q", cache, shape)
     w, sinks, accumulate = 0 if window is None else _count(window, "window", 1), _count(sinks, "sinks"), 1 if accumulate else 0
     if accumulate and cache.weight is None:

@@ -7,6 +7,7 @@ import os as _os
 from collections import namedtuple
 
 import torch
+import torch.autograd.forward_ad as _fwd_ad
 from torch.autograd import Function as _TorchFunction
 from torch.autograd.function import once_differentiable
 
@@ -70,6 +71,15 @@ def _any_b16(args):
     return False
 
 
+def _no_tangents(name, ts):
+    """Refuses inputs that carry a forward-mode derivative: no op of this package has one, and a forward that runs without torch's own
+    ``apply`` would drop it without a word."""
+    if _fwd_ad._current_level >= 0:   # (inside a dual_level)
+        for t in ts:
+            if torch.is_tensor(t) and _fwd_ad.unpack_dual(t).tangent is not None:
+                raise _lib.HipLibraryError("%s has no forward-mode derivative, and an input carries a tangent" % name)
+
+
 class Function(_TorchFunction):
     """torch.autograd.Function plus ``call``: inside backward passes that are not themselves recorded (grad mode off:
     the final second-order / first-order backward) the nested nodes skip the autograd bookkeeping and run their
@@ -95,6 +105,7 @@ class Function(_TorchFunction):
     def call(cls, *args):
         if torch.is_grad_enabled():
             return cls.apply(*args)
+        _no_tangents(cls.__name__, args)
         if _b16_seen[0] and cls.b16 != "native" and _any_b16(args):
             from .. import b16
             if cls.b16_twin is not None and _B16_TWINS:
