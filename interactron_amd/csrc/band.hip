@@ -1093,7 +1093,7 @@ int band_of(BandArgs& a, const ix_band* s, const char* who) {
     IX_CHECK_ARG(s->heads > 0 && s->kv_heads > 0 && s->heads % s->kv_heads == 0, "%s: %d query heads over %d key heads", who, s->heads, s->kv_heads);
     IX_CHECK_ARG((int64_t)s->batch * s->heads < kMostGroups, "%s: too many heads", who);
     IX_CHECK_ARG(s->window >= 0 && s->sinks >= 0, "%s: negative window or sinks", who);
-    IX_CHECK_ARG(s->scale == s->scale && s->scale < INFINITY && s->scale > -INFINITY, "%s: the scale is no number", who);
+    IX_CHECK_ARG(seq_scale_ok(s->scale), "%s: the scale is no number, or too large", who);
     IX_CHECK_ARG(s->q && s->k && s->v && ix_al16(s->q) && ix_al16(s->k) && ix_al16(s->v), "%s: null or unaligned q, k or v", who);
     const int64_t eb = s->dtype == 0 ? 4 : 2;
     for (int64_t x : {s->q_sb, s->q_sl, s->q_sh, s->k_sb, s->k_sl, s->k_sh, s->v_sb, s->v_sl, s->v_sh})

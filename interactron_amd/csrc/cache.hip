@@ -738,6 +738,7 @@ extern "C" int ix_cache_attn(const struct ix_paged_cache* cache, const void* q, 
     const int eb = cache->dtype == 0 ? 4 : 2, hd = cache->hd;
     IX_CHECK_ARG(q && out && ix_al16(q) && ix_al16(out) && sq_b * eb % 16 == 0 && sq_h * eb % 16 == 0, "ix_cache_attn: null or unaligned query or output");
     IX_CHECK_ARG(!accumulate || cache->weight, "ix_cache_attn: accumulate without weights in the cache");
+    IX_CHECK_ARG(seq_scale_ok(scale), "ix_cache_attn: the scale is no number, or too large");
     const Plan r = plan_of(cache, heads, window, sinks, accumulate);
     const size_t need = 4 * (r.o + r.ml + r.logits);
     if (need && (!workspace || workspace_bytes < need)) {

@@ -14,6 +14,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 #define SEQ_LOG2E 1.4426950408889634f
+// exponents are taken to base 2: a scale whose product with log2(e) is no finite float32 would turn scores of zero into NaN
+static inline bool seq_scale_ok(float scale) { return scale * SEQ_LOG2E < INFINITY && scale * SEQ_LOG2E > -INFINITY; }
 
 template <int DT> struct SeqT { typedef unsigned short elem; static constexpr int bytes = 2, words = 4; };   // words: registers of eight elements
 template <> struct SeqT<0> { typedef float elem; static constexpr int bytes = 4, words = 8; };

@@ -9,7 +9,7 @@ import struct
 import torch
 
 from .. import _lib
-from .cache import _DTYPES, _HEAD_DIMS, _count, _here
+from .cache import _DTYPES, _HEAD_DIMS, _count, _here, _scale
 from .core import Function, _L, _NullCtx, _chk
 
 
@@ -129,7 +129,4 @@ def band_attention(q, k, v, window=None, sinks=0, causal=True, scale=None, q_len
         if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):
             raise ValueError("%s must be a contiguous int32 [%d], got %s %s" % (name, B, t.dtype, list(t.shape)))
     window, sinks = 0 if window is None else _count(window, "window", 1), _count(sinks, "sinks")
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not abs(scale) < 3e38:   # (a float32, and no NaN)
-        raise ValueError("scale must be a finite number, got %r" % scale)
-    return BandAttention.call(q, k, v, q_lens, kv_lens, window, sinks, 1 if causal else 0, scale)
+    return BandAttention.call(q, k, v, q_lens, kv_lens, window, sinks, 1 if causal else 0, _scale(scale, D))

@@ -69,6 +69,14 @@ def _count(x, name, least=0):
     return x
 
 
+def _scale(scale, hd):
+    """A softmax's factor; exponents are taken to base 2, so scale log2(e) has to be a float32 too"""
+    scale = hd ** -0.5 if scale is None else float(scale)
+    if not abs(scale) < 2.35e38:   # (and no NaN)
+        raise ValueError("scale must be a finite number below 2.35e38, got %r" % scale)
+    return scale
+
+
 class PagedCache:
     """Keys and values of `batch` sequences in pages of a shared pool.
 
@@ -204,9 +212,7 @@ def cache_attention(q, cache, scale=None, window=None, sinks=0, accumulate=False
     w, sinks, accumulate = 0 if window is None else _count(window, "window", 1), _count(sinks, "sinks"), 1 if accumulate else 0
     if accumulate and cache.weight is None:
         raise ValueError("accumulate: the cache holds no weights")
-    scale = cache.hd ** -0.5 if scale is None else float(scale)
-    if not abs(scale) < 3e38:   # (a float32, and no NaN)
-        raise ValueError("scale must be a finite number, got %r" % scale)
+    scale = _scale(scale, cache.hd)
     s = _here(("q",), q)
     out, ws, need = q.new_empty(shape), None, _attention_ws(cache, H, w, sinks, accumulate)
     if need:   # (a buffer per call: calls on other streams and captured graphs share none)
