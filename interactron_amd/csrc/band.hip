@@ -204,7 +204,7 @@ struct BandArgs {
     float *lse, *delta, *part, *part_ml, *part_q;             // [B][H][Lp] base-2 normalisers (+inf: nothing visible) and delta; partial sums
     const int *q_lens, *kv_lens;
     int B, Lq, Lk, Lp, H, kv, left, right, sinks, causal;
-    int wide_blocks, wide_splits, splits, key_groups;         // dk / dv: see the host side; workgroups of theirs
+    int wide_blocks, wide_splits, splits, key_groups, cut;    // dk / dv: see the host side; workgroups of theirs; of a (batch, key head) cut blocks have
     int q_splits;                                             // dq: pieces of a block's key tiles
     int fwd_splits;                                           // forward: pieces of a block's key tiles
     float c2, scale;                                          // |scale| log2(e), scale
@@ -914,7 +914,7 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
             for (int db = 0; db < I::DB; ++db) ak[nb][db] = av[nb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         if (it.splits > 1) {
-            float* dst = a.part + (((int64_t)bk * (a.key_groups / (a.B * a.kv)) + item) * 2 * ROWS + row) * D;
+            float* dst = a.part + (((int64_t)bk * a.cut + item) * 2 * ROWS + row) * D;
 #pragma unroll
             for (int db = 0; db < I::DB; ++db) {
                 *reinterpret_cast<f32x4*>(dst + 16 * db + 4 * g) = ak[nb][db] * fk;
@@ -950,7 +950,7 @@ __global__ __launch_bounds__(kBlock, 2) void band_bwd_kernel(BandArgs a) {
 
 // dk, dv (and, with pieces of dq, then dq) of the blocks that were cut: the partial sums in their order, four values a thread
 template <int DT, int D>
-__global__ __launch_bounds__(kBlock) void band_sum_kernel(BandArgs a, int items, int rows) {
+__global__ __launch_bounds__(kBlock) void band_sum_kernel(BandArgs a, int rows) {
     typedef Img<DT, D> I;
     const int block = blockIdx.y;
     if ((int)blockIdx.x >= a.B * a.kv) {
@@ -975,7 +975,7 @@ __global__ __launch_bounds__(kBlock) void band_sum_kernel(BandArgs a, int items,
     for (int e = (blockIdx.z * kBlock + threadIdx.x) * 4; e < 2 * rows * D; e += gridDim.z * kBlock * 4) {
         const int which = e / (rows * D), row = e / D % rows, d = e % D, j = block * rows + row;
         if (j >= a.Lk) continue;
-        const float* src = a.part + ((int64_t)bk * items + item) * 2 * rows * D + e;
+        const float* src = a.part + ((int64_t)bk * a.cut + item) * 2 * rows * D + e;
         f32x4 x = *reinterpret_cast<const f32x4*>(src);
 #pragma unroll 8
         for (int s = 1; s < splits; ++s) x += *reinterpret_cast<const f32x4*>(src + (int64_t)s * 2 * rows * D);
@@ -1030,7 +1030,7 @@ size_t fwd_part(const ix_band* s) {   // partial rows
     return r == 1 ? 0 : (size_t)s->batch * s->heads * s->Lq * r;
 }
 
-struct KeyPlan { int blocks, wide, wide_splits, splits, items; };
+struct KeyPlan { int blocks, wide, wide_splits, splits, items, cut; };   // cut: how many of the items leave partial sums (they come first)
 
 // Pieces of every block in the backward pass, of `wgs` blocks (of keys for dk / dv, of queries for dq) that stream `tiles` tiles of `tb` rows.
 // Fewer blocks than compute units (few heads, or few key heads): about 384 pieces of at least four tiles.  Fewer than two a unit: two pieces of
@@ -1063,6 +1063,7 @@ KeyPlan key_plan(const ix_band* s) {
     if (ws < r.splits) ws = r.splits;
     r.wide_splits = (int)(ws > 64 ? 64 : ws);
     r.items = r.wide * r.wide_splits + (r.blocks - r.wide) * r.splits;
+    r.cut = r.splits > 1 ? r.items : r.wide_splits > 1 ? r.wide * r.wide_splits : 0;
     return r;
 }
 
@@ -1077,10 +1078,7 @@ size_t dq_part_bytes(const ix_band* s) {
     return r == 1 ? 0 : (size_t)s->batch * s->heads * div_up(s->Lq, rows) * r * rows * s->hd * 4;
 }
 
-size_t part_bytes(const ix_band* s, const KeyPlan& r) {
-    if (r.splits == 1 && (r.wide_splits == 1 || r.wide == 0)) return 0;
-    return (size_t)s->batch * s->kv_heads * r.items * 2 * owner_rows(bwd_nb(s)) * s->hd * 4;
-}
+size_t part_bytes(const ix_band* s, const KeyPlan& r) { return (size_t)s->batch * s->kv_heads * r.cut * 2 * owner_rows(bwd_nb(s)) * s->hd * 4; }
 
 int64_t lse_pitch(const ix_band* s) { return ((int64_t)s->Lq + 127) / 128 * 128; }
 
@@ -1222,6 +1220,7 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
     a.wide_blocks = r.wide;
     a.wide_splits = r.wide_splits;
     a.splits = r.splits;
+    a.cut = r.cut;
     const int nb = bwd_nb(s), rows = owner_rows(nb);
     const int64_t key_groups = (int64_t)a.B * a.kv * r.items, groups = key_groups + (int64_t)a.B * a.H * ((a.Lq + rows - 1) / rows) * a.q_splits;
     const int64_t delta_groups = ((int64_t)a.B * a.H * a.Lp * (s->hd * eb / 16) + kBlock - 1) / kBlock;
@@ -1236,7 +1235,7 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
     if (parts || parts_q) {
         const int k_blocks = r.splits > 1 ? r.blocks : parts ? r.wide : 0, q_blocks = parts_q ? (a.Lq + rows - 1) / rows : 0;   // (both under 65 536)
         const dim3 sgrid(a.B * (a.kv + (parts_q ? a.H : 0)), k_blocks > q_blocks ? k_blocks : q_blocks, 4);
-#define BAND_SUM(DT, D) band_sum_kernel<DT, D><<<sgrid, kBlock, 0, stream>>>(a, r.items, rows)
+#define BAND_SUM(DT, D) band_sum_kernel<DT, D><<<sgrid, kBlock, 0, stream>>>(a, rows)
         BAND_GO(BAND_SUM)
         IX_CHECK_LAUNCH("ix_band_attn_bwd (sum)");
     }
