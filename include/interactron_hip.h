@@ -543,7 +543,9 @@ int ix_adam_step_f32(float* p, float* g, float* m, float* v, int64_t n, float lr
  *                      from ix_band_attn_lse_pitch), and rest like out: what its rounding to 16 bits took away (not with f32).  Few
  *                      rows over many keys go in pieces that are joined: workspace of ix_workspace_bytes_band_attn_fwd bytes (often 0)
  *   ix_band_attn_bwd : dq, dk, dv (dense, like q, k, v) from out, rest, lse and d_out [batch][Lq][heads][hd] by strides g_*; sums in f32,
- *                      in a fixed order (no atomics); workspace of ix_workspace_bytes_band_attn_bwd bytes, 16-byte aligned */
+ *                      in a fixed order (no atomics); workspace of ix_workspace_bytes_band_attn_bwd bytes, 16-byte aligned
+ *   ix_band_attn_bwd_some : the same for some of them: want 1 dq, 2 dk and dv, 3 all (the same bits); what is not wanted is not computed and
+ *                      its pointers are not looked at */
 struct ix_band {
     const void *q, *k, *v;
     int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
@@ -558,6 +560,9 @@ int ix_band_attn_lse_pitch(int Lq, int64_t* out_host);
 int ix_workspace_bytes_band_attn_bwd(const struct ix_band* band_host, size_t* out_host);
 int ix_band_attn_bwd(const struct ix_band* band_host, const void* out, const void* rest, const float* lse, const void* d_out, int64_t g_sb,
                      int64_t g_sl, int64_t g_sh, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, ix_stream_t stream);
+int ix_band_attn_bwd_some(const struct ix_band* band_host, int want, const void* out, const void* rest, const float* lse, const void* d_out,
+                          int64_t g_sb, int64_t g_sl, int64_t g_sh, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                          ix_stream_t stream);
 
 /* ---- A paged cache of keys and values (csrc/cache.hip): acting on a rollout that grows token by token --------------------------------
  * The reference runs its fusion transformer over the whole sequence again for every new frame (models/transformer.py:49-60,

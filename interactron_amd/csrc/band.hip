@@ -1190,17 +1190,22 @@ extern "C" int ix_workspace_bytes_band_attn_bwd(const struct ix_band* s, size_t*
     return IX_OK;
 }
 
-extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const void* rest, const float* lse, const void* d_out, int64_t g_sb, int64_t g_sl,
-                                int64_t g_sh, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+extern "C" int ix_band_attn_bwd_some(const struct ix_band* s, int want, const void* out, const void* rest, const float* lse, const void* d_out, int64_t g_sb,
+                                     int64_t g_sl, int64_t g_sh, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                     hipStream_t stream) {
     BandArgs a;
     if (int rc = band_of(a, s, "ix_band_attn_bwd")) return rc;
+    IX_CHECK_ARG(want >= 1 && want <= 3, "ix_band_attn_bwd: want %d is none of 1 (dq), 2 (dk and dv), 3", want);
+    const bool to_q = want & 1, to_k = want & 2;
+    if (!to_q) dq = nullptr;
+    if (!to_k) dk = dv = nullptr;
     const int64_t eb = s->dtype == 0 ? 4 : 2;
-    IX_CHECK_ARG(out && (rest || s->dtype == 0) && lse && d_out && dq && dk && dv, "ix_band_attn_bwd: null pointer");
+    IX_CHECK_ARG(out && (rest || s->dtype == 0) && lse && d_out && (dq || !to_q) && ((dk && dv) || !to_k), "ix_band_attn_bwd: null pointer");
     IX_CHECK_ARG(ix_al16(out) && ix_al16(rest) && ix_al16(d_out) && ix_al16(dq) && ix_al16(dk) && ix_al16(dv), "ix_band_attn_bwd: unaligned pointer");
     for (int64_t x : {g_sb, g_sl, g_sh}) IX_CHECK_ARG(x * eb % 16 == 0, "ix_band_attn_bwd: rows that do not start on 16 bytes");
     IX_CHECK_ARG(g_sl >= 0 && g_sl * eb < (1 << 24), "ix_band_attn_bwd: rows 2^24 bytes apart or more");
-    const KeyPlan r = key_plan(s);
-    const size_t parts = part_bytes(s, r), parts_q = dq_part_bytes(s), need = (size_t)a.B * a.H * a.Lp * 4 + parts + parts_q;
+    const KeyPlan r = to_k ? key_plan(s) : KeyPlan{0, 0, 1, 1, 0, 0};   // (no blocks of keys: none of them cut)
+    const size_t parts = part_bytes(s, r), parts_q = to_q ? dq_part_bytes(s) : 0, need = (size_t)a.B * a.H * a.Lp * 4 + parts + parts_q;
     if (!workspace || workspace_bytes < need || !ix_al16(workspace)) {
         ix_set_error("ix_band_attn_bwd: workspace of %zu bytes (16-byte aligned), %zu needed", workspace ? workspace_bytes : (size_t)0, need);
         return IX_ERR_WORKSPACE;
@@ -1222,7 +1227,7 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
     a.splits = r.splits;
     a.cut = r.cut;
     const int nb = bwd_nb(s), rows = owner_rows(nb);
-    const int64_t key_groups = (int64_t)a.B * a.kv * r.items, groups = key_groups + (int64_t)a.B * a.H * ((a.Lq + rows - 1) / rows) * a.q_splits;
+    const int64_t key_groups = (int64_t)a.B * a.kv * r.items, groups = key_groups + (to_q ? (int64_t)a.B * a.H * ((a.Lq + rows - 1) / rows) * a.q_splits : 0);
     const int64_t delta_groups = ((int64_t)a.B * a.H * a.Lp * (s->hd * eb / 16) + kBlock - 1) / kBlock;
     IX_CHECK_ARG(groups < kMostGroups && delta_groups < kMostGroups, "ix_band_attn_bwd: too many rows for one launch");
     a.key_groups = (int)key_groups;
@@ -1240,4 +1245,9 @@ extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const 
         IX_CHECK_LAUNCH("ix_band_attn_bwd (sum)");
     }
     return IX_OK;
+}
+
+extern "C" int ix_band_attn_bwd(const struct ix_band* s, const void* out, const void* rest, const float* lse, const void* d_out, int64_t g_sb, int64_t g_sl,
+                                int64_t g_sh, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    return ix_band_attn_bwd_some(s, 3, out, rest, lse, d_out, g_sb, g_sl, g_sh, dq, dk, dv, workspace, workspace_bytes, stream);
 }

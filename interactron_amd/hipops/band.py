@@ -93,11 +93,14 @@ class BandAttention(Function):
         band, n = _band(q, k, v, q_lens, kv_lens, *ctx.how), ctypes.c_size_t(0)
         _chk(_L().ix_workspace_bytes_band_attn_bwd(band, ctypes.byref(n)), "ix_workspace_bytes_band_attn_bwd")
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        dq, dk, dv = _like(q), _like(k), _like(v)
+        want = (1 if need[0] else 0) | (2 if need[1] or need[2] else 0)   # (dk and dv come together)
+        if not want:
+            return (None,) * 9
+        dq, dk, dv = _like(q) if want & 1 else None, _like(k) if want & 2 else None, _like(v) if want & 2 else None
         lse, (gb, gl, gh, _) = kept.data_ptr(), do.stride()
         rest = None if q.dtype is torch.float32 else lse + kept.numel() - 2 * q.numel()
-        _chk(_L().ix_band_attn_bwd(band, out.data_ptr(), rest, lse, do.data_ptr(), gb, gl, gh, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(),
-                                   n.value, s), "ix_band_attn_bwd")
+        _chk(_L().ix_band_attn_bwd_some(band, want, out.data_ptr(), rest, lse, do.data_ptr(), gb, gl, gh, _ptr(dq), _ptr(dk), _ptr(dv), ws.data_ptr(),
+                                        n.value, s), "ix_band_attn_bwd_some")
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None, None, None
 
 
