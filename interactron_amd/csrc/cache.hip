@@ -638,6 +638,19 @@ int cache_of(Cache& c, const ix_paged_cache* s, const char* who) {
     return IX_OK;
 }
 
+// Memory of the pools, and of rows [batch][T][kv][row] by byte strides: whether they share any.
+struct Span { const unsigned char *from, *to; };
+Span pool_span(const ix_paged_cache* s, const void* pool) {
+    const unsigned char* p = static_cast<const unsigned char*>(pool);
+    return Span{p, p + s->pages_total * s->kv_heads * s->page * s->hd * (s->dtype == 0 ? 4 : 2)};
+}
+Span row_span(const ix_paged_cache* s, const void* rows, int64_t T, int64_t sb, int64_t st, int64_t sh) {
+    Span r{static_cast<const unsigned char*>(rows), static_cast<const unsigned char*>(rows) + s->hd * (s->dtype == 0 ? 4 : 2)};
+    for (int64_t far : {(s->batch - 1) * sb, (T - 1) * st, (s->kv_heads - 1) * sh}) (far < 0 ? r.from : r.to) += far;
+    return r;
+}
+bool meet(const Span& a, const Span& b) { return a.from < b.to && b.from < a.to; }
+
 struct Plan {   // of one attention launch
     int max_tiles, splits, least, qtiles, kt, waves;
     bool join;
@@ -700,6 +713,10 @@ extern "C" int ix_cache_append(const struct ix_paged_cache* cache, const void* k
     for (int64_t s : {sb_k, st_k, sh_k, sb_v, st_v, sh_v}) IX_CHECK_ARG(s * eb % 16 == 0, "ix_cache_append: rows that do not start on 16 bytes");
     for (const int* x : {counts, at})   // (the lengths themselves may be named; another part of their memory would change under the call)
         IX_CHECK_ARG(!x || x == c.lens || x + c.batch <= c.lens || c.lens + c.batch <= x, "ix_cache_append: counts or at overlap the lengths");
+    const Span pool_k = pool_span(cache, cache->k), pool_v = pool_span(cache, cache->v);
+    IX_CHECK_ARG(!meet(pool_k, pool_v), "ix_cache_append: keys and values share memory");
+    for (const Span& x : {row_span(cache, k, T, sb_k * eb, st_k * eb, sh_k * eb), row_span(cache, v, T, sb_v * eb, st_v * eb, sh_v * eb)})
+        IX_CHECK_ARG(T == 0 || !(meet(x, pool_k) || meet(x, pool_v)), "ix_cache_append: the new rows are parts of the cache's own pools");
     AppendArgs p{c, static_cast<const unsigned char*>(k), static_cast<const unsigned char*>(v), sb_k * eb, st_k * eb, sh_k * eb, sb_v * eb, st_v * eb,
                  sh_v * eb, counts, at, T, cache->hd * eb / 16, 0, 0};
     // a workgroup moves up to 1 024 16-byte chunks of K and as many of V: four of each per thread
@@ -801,6 +818,7 @@ extern "C" int ix_cache_compact(const struct ix_paged_cache* cache, const int* k
     if (int rc = cache_of(p.c, cache, "ix_cache_compact")) return rc;
     IX_CHECK_ARG(kept && left && budget > 0, "ix_cache_compact: null pointer or empty budget");
     IX_CHECK_ARG(left + cache->batch <= cache->lens || cache->lens + cache->batch <= left, "ix_cache_compact: the new lengths overlap the cache's own");
+    IX_CHECK_ARG(!meet(pool_span(cache, cache->k), pool_span(cache, cache->v)), "ix_cache_compact: keys and values share memory: rows would move twice");
     p.kept = kept;
     p.left = left;
     p.budget = budget;

@@ -158,8 +158,9 @@ def cache_append(cache, k, v, counts=None, at=None):
     """Writes k, v [B, T, kv_heads, hd] as tokens at[b] .. at[b] + counts[b] - 1 of every sequence and sets the lengths to at + counts.
 
     at: int32 [B], default: the cache's lengths (the new tokens follow the old ones; an earlier place takes tokens back, behind a later one
-    lies whatever the pages held).  counts: int32 [B], default T (rows behind a sequence's count are padding and not read).  Tokens beyond the capacity are dropped.  New tokens have
-    had no attention yet: their weight is 0.  k and v must not be parts of the cache's own pools."""
+    lies whatever the pages held).  counts: int32 [B], default T (rows behind a sequence's count are padding and not read).  Tokens beyond
+    the capacity are dropped.  New tokens have had no attention yet: their weight is 0.  k and v must not be parts of the cache's own pools, nor
+    the pools of each other."""
     if k.dim() != 4:
         raise ValueError("new keys must be [batch, tokens, kv_heads, hd], got %s" % list(k.shape))
     T = k.shape[1]
@@ -250,7 +251,7 @@ def cache_select(weight, lens, budget, sinks=0, recent=0):
 def cache_compact(cache, kept, left):
     """Moves the tokens kept[b, h, :left[b]] of every sequence and key head to its front, in place and in order, with their weights, and
     sets the lengths to left.  kept int32 [B, kv_heads, budget] ascends in every row (as cache_select returns it); the pages of a
-    sequence must be its own: no other sequence's table may name them."""
+    sequence must be its own: no other sequence's table may name them, and the pools must not share memory."""
     if kept.dim() != 3 or kept.shape[2] == 0:
         raise ValueError("kept must be [batch, kv_heads, budget], got %s" % list(kept.shape))
     _whole(kept, "kept", torch.int32, (cache.batch, cache.kv_heads, kept.shape[2]))
