@@ -532,13 +532,13 @@ int ix_adam_step_f32(float* p, float* g, float* m, float* v, int64_t n, float lr
                      int step, const float* sumsq, float max_norm, int zero_grad, ix_stream_t stream);
 
 /* ---- Band attention (csrc/band.hip): softmax(scale q k^T) v over a band around the diagonal and a few first keys ---------------------
- * The sliding form of the attention of models/gpt.py:39-57 and models/detr_models/transformer.py:148-161 for rollouts whose [L, S] is
- * too much: query i of a sequence of m queries and n keys stands at p = i + n - m and sees the keys j < n with |p - j| < window (0:
+ * The sliding form of the attention of models/gpt.py:39-57 and models/detr_models/transformer.py:148-161 for sequences whose [L, S] is
+ * too much (no dropout): query i of a sequence of m queries and n keys stands at p = i + n - m and sees the keys j < n with |p - j| < window (0:
  * all) or j < sinks; with `causal` also j <= p.  q [batch][Lq][heads][hd], k, v [batch][Lk][kv_heads][hd] by element strides (sb, sl,
  * sh; rows dense and on 16 bytes); query head h reads key head h / (heads / kv_heads).  dtype 0 f32, 1 bf16, 2 fp16; hd 32, 64, 128.
  * q_lens, kv_lens int32 [batch] (null: Lq, Lk): rows behind them are never read and come back as zeros.  A query that sees nothing
  * gives zeros and has no gradient.  Inside the lengths v has to be finite also where a query does not see it, for the gradients q, k
- * and d_out too.  batch * heads < 2^24.
+ * and d_out too.  batch * heads < 2^24; |scale| log2(e) is a finite float32.
  *   ix_band_attn_fwd : out [batch][Lq][heads][hd] dense; for the gradients (may be null) lse f32 [batch][heads][pitch], base 2 (pitch
  *                      from ix_band_attn_lse_pitch), and rest like out: what its rounding to 16 bits took away (not with f32).  Few
  *                      rows over many keys go in pieces that are joined: workspace of ix_workspace_bytes_band_attn_fwd bytes (often 0)
@@ -564,15 +564,15 @@ int ix_band_attn_bwd_some(const struct ix_band* band_host, int want, const void*
                           int64_t g_sb, int64_t g_sl, int64_t g_sh, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                           ix_stream_t stream);
 
-/* ---- A paged cache of keys and values (csrc/cache.hip): acting on a rollout that grows token by token --------------------------------
- * The reference runs its fusion transformer over the whole sequence again for every new frame (models/transformer.py:49-60,
- * models/interactron.py:166-190); these entry points keep what has been seen.  Token t of sequence b and key head h lives at row
+/* ---- A paged cache of keys and values (csrc/cache.hip): sequences that grow token by token --------------------------------------------
+ * For causal layers, where a token's keys and values stay what they were.  (The reference's fusion transformer is bidirectional: it runs over
+ * the whole sequence again for every new frame, models/transformer.py:49-60, models/interactron.py:166-190.)  Token t of sequence b and key head h lives at row
  * t % page of page table[b][t / page] in pools k, v [pages_total][kv_heads][page][hd].  dtype: 0 f32, 1 bf16, 2 fp16; hd 32, 64 or
  * 128; page a power of two, 16 .. 1024.  lens [batch]: tokens held (clamped to 0 .. pages * page).  weight [batch][kv_heads]
  * [pages * page] f32 (may be null): attention that every token has had so far.  A page id outside the pool is never dereferenced: its
  * tokens count as masked, what is written there is dropped.  Strides are in elements, rows start on 16 bytes.
  *   ix_cache_append : rows k, v [batch][T][kv_heads][hd] -> tokens at[b] .. at[b] + counts[b] - 1 (null: the lengths; T), their weight
- *                     = 0, lens[b] = at[b] + counts[b]; tokens beyond the capacity are dropped
+ *                     = 0, lens[b] = at[b] + counts[b]; tokens beyond the capacity are dropped.  The rows must not lie in the pools
  *   ix_cache_attn   : out[b][h] = sum_j P_j v_j, P = softmax_j(scale q[b][h] . k_j) for one query per sequence and head that stands at
  *                     the last token; window > 0: the last `window` tokens and the first `sinks` only.  Query head h reads key head
  *                     h / (heads / kv_heads).  accumulate: weight[j] += sum of P_j over the query heads of the key head.  An empty
@@ -581,7 +581,7 @@ int ix_band_attn_bwd_some(const struct ix_band* band_host, int want, const void*
  *                     the largest weight (NaN counts least; of equal weights the lowest index); all tokens, then -1, where there are
  *                     no more than `budget`.  left[b] = min(lens[b], budget)
  *   ix_cache_compact: rows kept[b][h][i] >= i (ascending; others are skipped) -> rows i < left[b], in place, with their weights;
- *                     lens = left */
+ *                     lens = left.  As for append, k and v must not share memory */
 struct ix_paged_cache {
     void *k, *v;
     const int* table;

@@ -192,8 +192,8 @@ template <int N> __device__ __forceinline__ void landed() {
     asm volatile("" ::: "memory");
 }
 // stages of the ring: three (requests two tiles ahead) where a workgroup's LDS stays within the limit, else two.  Gradients 48 KB; forward 32,
-// where one more workgroup fits on a compute unit instead (48 / 32 KB: f32 of 8 heads of 64, 8 192 with window 1 000 173 / 161 us; bf16, 12 755
-// with window 2 551 102 / 99.5, 2 x 2 060 with window 412 22.7 / 22.1, 2 x 4 096 in full 62.5 / 64).
+// where one more workgroup fits on a compute unit instead (48 / 32 KB: f32 of 8 heads of 64, 8 192 with window 1 000 167 / 153 us; bf16, 12 755
+// with window 2 551 128 / 130, 2 x 2 060 with window 412 24.2 / 24.0, 2 x 4 096 in full 69 / 70).
 constexpr int stages(int bytes, int limit) { return 3 * bytes <= limit ? 3 : 2; }
 constexpr int kFwdRing = 32768, kBwdRing = 49152;
 
@@ -347,10 +347,12 @@ constexpr float kFirstF = 1099511627776.f;   // 2^40
 // ====================================================================================================================================
 // The running maximum is raised only where a tile exceeds it by more than 2^8 (a weight may then reach 256, exact in all types' ranges):
 // most tiles leave the accumulators alone.  16-bit types: a weight goes into the second product as two terms (rest_frag), into the sum unrounded.
-// Bound by matrix and vector instructions together (matrix pipe 43 % and vector instructions 51 % of busy cycles at hd 128, 33 and 63 % at
-// hd 64, a tenth of the time for the bytes, no LDS conflicts): fp16, 8 192 queries and keys of 32 / 8 heads of 128, window 2 048: 275 us =
-// 875 TFLOP/s, 0.75 of what a plain product of 8 192^3 reaches; bf16, 12 755 of 8 heads of 64, window 2 551: 89-103 us = 580-680 TFLOP/s (a
-// score costs as much exponential for half the product); 2 060 of 16 heads of 64, window 412: 24 us, its 528 workgroups' first and last tiles.
+// 16-bit types are bound by matrix and vector instructions together (matrix pipe 54 % and vector instructions 54 % of busy cycles at hd 128, 37 and
+// 70 % at hd 64, no LDS conflicts): fp16, 8 192 queries and keys of 32 / 8 heads of 128, window 2 048: 342-358 us = 1 070-1 115 TFLOP/s over
+// three products, 0.92-0.96 of what a plain product of 8 192^3 reaches; bf16, 12 755 of 8 heads of 64, window 2 551: 119-130 us = 730-795 TFLOP/s
+// (a score costs as much exponential for half the product); 2 060 of 16 heads of 64, window 412: 24 us, its 528 workgroups' first and last
+// tiles.  f32, 16 x 361 of 8 heads of 32, window 64: 20 us = 52 of 154 TFLOP/s, matrix pipe 40 %, vector instructions 23 %, and of the LDS cycles
+// a quarter bank conflicts: six short tiles a workgroup do not cover their waits.
 constexpr float kSlack = 8.f;
 // fp16: weights are carried 2^7 and, for dv, 2^12 times as large (the largest forward weight, 2^8 by the slack, is then 2^15; the type ends at
 // 65 504), so that its smallest step, 2^-24, is 2^-31 of the row's largest weight and 2^-36: a row whose first key takes nearly all the weight
@@ -933,9 +935,10 @@ __device__ __forceinline__ void band_dkv(const BandArgs& a, unsigned char* mem, 
 
 // Both in one launch, the key blocks first: either alone would leave compute units empty at the sizes where time counts, and at its end.
 // Ten products of 2 hd operations a pair (four of the formulas, q k^T and do v^T twice, the second terms of P and dz): 12 755 queries and keys of 8
-// heads of 64, window 2 551, bf16: 307-343 us = 790-900 TFLOP/s, matrix pipe 43 % and vector instructions 56 % of busy cycles; head dim 128 at
-// 8 192 of 32 / 8 heads, window 2 048: 1 317 us = 820 TFLOP/s; f32, 16 x 361 of 8 heads of 32, window 64: 47 us.  Scores of the next 32 rows
-// ahead of this one's exponentials: 350 / 350 us.
+// heads of 64, window 2 551, bf16: 300 us (353 under a profiler) = 1 050 TFLOP/s, matrix pipe 44 % and vector instructions 58 % of busy cycles;
+// 2 x 2 060, window 412: 57-64 us = 460-520 TFLOP/s, 1 056 workgroups in 768 places; head dim 128 at 8 192 of 32 / 8 heads, window 2 048: 1 200
+// us; f32 (seven products), 16 x 361 of 8 heads of 32, window 64: 48 us = 72 TFLOP/s, matrix pipe 55 %, vector instructions 20 %.  Scores of
+// the next 32 rows ahead of this one's exponentials gained nothing (350 / 350 us before the weights had a second term).
 template <int DT, int D> constexpr int bwd_bytes() {
     constexpr int qs = 2 * key_tile(DT) * Img<DT, D>::ROW, ks = 2 * query_tile(DT, D) * Img<DT, D>::ROW;
     constexpr int q = stages(qs, kBwdRing) * qs, k = stages(ks, kBwdRing) * (ks + 1024);
@@ -994,10 +997,11 @@ int64_t reach(const ix_band* s) {   // rows on both sides that a band takes from
 
 // Owner rows: 64 or 128 a workgroup (one or two blocks of 16 for every wave).  Two blocks read LDS half as often for the same products, one
 // gives twice as many workgroups and waves, and evens out the lengths of causal rows.  Measured, bf16 (us, one / two, by the number of
-// workgroups of 128 rows): forward head dim 64, 64: 9 / 13, 272: 24 / 28, 800: 120 / 105; head dim 32, 544: 27 / 30, 1 024: 142 / 132; head dim
-// 128, where LDS counts double, 64: 14 / 18, 256: 25 / 31 causal and 30 / 32 not, 384: 40 / 46 causal but 68 / 60 not and 28 / 25 with a window,
-// 448: 48 / 50, 85 / 69 and 48 / 42, 512: 66 / 57, 2 048: 399 / 310.  Gradients head dim 64, 192: 12.6 / 15, 576: 49 / 49, 1 632: 322 / 284; head
-// dim 128 only one (two take the registers of a second wave: 20 / 37 at 176, 667 / 913 at 2 048).  f32 has room for one.
+// workgroups of 128 rows): forward head dim 64, 64: 15 / 25, 272: 34 / 48, 800: 122 / 119 (12 755 rows) and, of 800-row sequences, 28 / 33;
+// head dim 32, 576: 21 / 25, 1 024: 50 / 49, 800: 92 / 101 (12 755 rows); head dim 128, where LDS counts double, 64: 23 / 33, 256: 26 / 34
+// causal and 33 / 35 not, 384: 39 / 51 causal but 72 / 68 not and 31 / 30 with a window, 448: 61 / 66, 111 / 92 and 35 / 35, 512: 66 / 68, 114 / 96
+// and 38 / 35, 2 048: 392 / 331.  Gradients (with the forward) head dim 64, 192: 44 / 48, 576: 68 / 75, 1 152: 162 / 161, 1 600: 444 / 427; head
+// dim 128 only one (two take the registers of a second wave).  f32 has room for one.
 int fwd_nb(const ix_band* s) {
     if (s->dtype == 0) return 1;
     const int few = s->hd < 128 ? 600 : s->causal && s->window == 0 ? 512 : 384;
@@ -1010,11 +1014,10 @@ int bwd_nb(const ix_band* s) {
 
 // Pieces of the forward's key tiles: where the blocks of queries are fewer than two a compute unit, about 512 in all, up to 32 of a block and
 // at least four tiles each (eight where more than half of the units have a block: the join costs 4 to 5 us).  One piece / these: bf16, 40
-// queries of 16 heads of 128 over 6 000 keys 101 / 19 us, 6 000 of 2 heads of 64 72 / 35, 3 000 of 4 heads 38 / 24, 4 x 512 of 8 heads of 128
-// over 8 192 keys 145 / 115; f32, 4 096 of 4 heads of 64 185 / 145; fp16, 8 192 of 2 heads of 128 136 / 95.  No gain: two pieces of five
-// tiles (3 000 of 4 heads, window 500) 11 / 15, of sixteen (2 060 of 8 heads of 64) 29.5 / 31.  About 768 pieces: 74 us for the 8 192 of 2
-// heads, but 124 for the 4 x 512.  Blocks of 128 rows, of which a compute unit holds half as many, stay whole (384 of them with 1 536 keys of hd
-// 128 46 / 58, 448 with window 512 42 / 65).
+// queries of 16 heads of 128 over 6 000 keys 119 / 21 us, 6 000 of 2 heads of 64 83 / 42, 3 000 of 4 heads 44 / 27, 4 x 512 of 8 heads of 128
+// over 8 192 keys 160 / 123; fp16, 8 192 of 2 heads of 128 153 / 113; f32, 4 096 of 4 heads of 64 185 / 145.  No gain: sixteen tiles (2 060 of 8
+// heads of 64) 31.4 / 30.6.  About 768 pieces: 88 us for the 8 192 of 2 heads, but 128 for the 4 x 512.  Blocks of 128 rows, of which a compute
+// unit holds half as many, stay whole (384 of them with 1 536 keys of hd 128 54 / 57).
 int fwd_splits(const ix_band* s) {
     const int64_t groups = (int64_t)s->batch * s->heads * div_up(s->Lq, owner_rows(fwd_nb(s)));
     if (groups >= 512 || fwd_nb(s) == 2) return 1;
@@ -1033,11 +1036,12 @@ size_t fwd_part(const ix_band* s) {   // partial rows
 struct KeyPlan { int blocks, wide, wide_splits, splits, items, cut; };   // cut: how many of the items leave partial sums (they come first)
 
 // Pieces of every block in the backward pass, of `wgs` blocks (of keys for dk / dv, of queries for dq) that stream `tiles` tiles of `tb` rows.
-// Fewer blocks than compute units (few heads, or few key heads): about 384 pieces of at least four tiles.  Fewer than two a unit: two pieces of
-// at least 1 536 rows.  Forward and gradients, us: uncut / with 256 / 384 / 512 pieces, f32, 2 x 2 041 of 2 heads of 64 234 / 180 / 146 / 145,
-// 6 000 of one head of 128 977 / 580 / 437 / 453; bf16, 40 queries of 16 heads over 6 000 keys of 4 of 128 159 / 58 / 57 / 68.  256 blocks, one
-// piece / two: 8 192 of 2 heads of 128 429 / 308, 4 096 of 4 heads of 64 in f32 610 / 455, 4 x 512 of 8 heads over 8 192 keys 533 / 461 -- but
-// 2 060 of 8 heads of 64 94 / 100, of 12 heads with window 800 60 / 72.
+// Fewer blocks than compute units (few heads, or few key heads): about 384 pieces, no more than one for every four tiles begun (five tiles
+// may become a piece of two and one of three).  Fewer than two a unit: two pieces of at least 1 536 rows.  Forward and gradients, us: uncut /
+// with 256 / 384 / 512 pieces, f32, 2 x 2 041 of 2 heads of 64 207 / 178 / 141 / 136, 6 000 of one head of 128 933 / 556 / 413 / 429; bf16, the same
+// 73 / 60 / 57 / 52 and 272 / 135 / 113 / 113, 40 queries of 16 heads over 6 000 keys of 4 of 128 167 / 63 / 60 / 60.  256 to 511 blocks, one piece /
+// two: 8 192 of 2 heads of 128 459 / 329, 4 096 of 4 heads of 64 in f32 621 / 457, 4 x 512 of 8 heads over 8 192 keys 572 / 495; shorter rows stay
+// whole: of 12 heads of 2 060, window 800, 59 / 66, though of 8 heads in full 85 / 76.
 int64_t bwd_pieces(int64_t wgs, int64_t tiles, int tb) {
     int64_t r = wgs < 256 ? div_up(384, wgs) : wgs < 512 ? 2 : 1;
     const int64_t most = wgs < 256 ? div_up(tiles, 4) : tiles * tb / 1536;

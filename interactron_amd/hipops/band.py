@@ -1,7 +1,10 @@
 """hipops.band -- attention over a band around the diagonal and a few first keys, with its gradients (csrc/band.hip).
 
-The sliding form of hipops.attention for rollouts that are too long to attend to in full (reference models/gpt.py:39-57 and
+The sliding form of hipops.attention for sequences that are too long to attend to in full (reference models/gpt.py:39-57 and
 models/detr_models/transformer.py:148-161 attend to everything): 16-bit or 32-bit rows as they are, shared key heads, padded batches.
+
+It is no drop-in for hipops.attention inside the package's own models, and none of them calls it: the fusion transformer trains with dropout on
+the weights, which this has not, and its inner gradient is differentiated again, which this refuses.
 """
 import ctypes
 import struct
@@ -112,8 +115,9 @@ def band_attention(q, k, v, window=None, sinks=0, causal=True, scale=None, q_len
     head h reads key head h // (heads // kv_heads).  scale: default 1 / sqrt(hd).  q_lens, kv_lens: int32 [B], the lengths m and n of a
     padded batch; padding is never read and comes back as zeros.  A query that sees nothing gives zeros and has no gradient.
 
-    float32, bfloat16 or float16 with sums and softmax in 32 bits, hd 32, 64 or 128, rows with any strides (a slice of a packed projection
-    is taken as it is).  Differentiable once.  Inside the lengths, values have to be finite also where a query does not see them, and for the
+    float32, bfloat16 or float16, hd 32, 64 or 128, rows with any strides (a slice of a packed projection is taken as it is).  Sums and softmax
+    are in 32 bits; 16-bit types carry weights and score gradients into the products as two terms of the type, so that results are off by their
+    own rounding.  No dropout.  Differentiable once, computing only the gradients that are needed (those of k and v together).  Inside the lengths, values have to be finite also where a query does not see them, and for the
     gradients queries, keys and the gradient of the output too: there a weight of zero is multiplied with them.  A captured backward pass
     has leaves of its own: no eager graph of the same leaves may be alive."""
     for t, name in ((q, "q"), (k, "k"), (v, "v")):

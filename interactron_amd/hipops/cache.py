@@ -1,5 +1,5 @@
-"""hipops.cache -- a paged cache of keys and values for acting on a rollout that grows token by token: writing new tokens, attention of
-one new token per sequence, and cutting the cache back to the tokens that have had the most attention (csrc/cache.hip).
+"""hipops.cache -- a paged cache of keys and values for sequences that grow token by token: writing new tokens, attention of one new token
+per sequence, and cutting the cache back to the tokens that have had the most attention (csrc/cache.hip).
 
     cache = hipops.PagedCache(k, v, table, lens, weight)      # tensors of the caller; nothing is copied
     hipops.cache_append(cache, new_k, new_v)                  # [B, T, kv_heads, hd] each, at the end of every sequence
@@ -7,8 +7,13 @@ one new token per sequence, and cutting the cache back to the tokens that have h
     hipops.cache_evict(cache, budget, sinks=4, recent=256)    # in place; the pages behind the budget are free again
 
 None of these has a backward.  All of them are ordered on the current stream, never wait for the GPU, take their sizes from the shapes
-alone (the lengths stay on the device) and may be captured into a HIP graph.  (The reference keeps nothing: it runs its fusion transformer
-over all frames again for every new one, models/interactron.py:166-190.)
+alone (the lengths stay on the device; a call's pieces and workspace follow the table's capacity, so a table much larger than the lengths costs
+a second launch) and may be captured into a HIP graph.
+
+For stacks of causal layers, where a token's keys and values stay what they were when it came.  The package's own fusion transformer is none:
+every token attends to all frames, so a new frame changes the earlier tokens from the second layer on, and it is run over all frames again
+(reference models/interactron.py:166-190); no model of the package holds a cache.  Several new tokens of a sequence at once attend through
+band_attention over dense keys.
 """
 import ctypes
 
