@@ -396,7 +396,7 @@ def capture_begin(salt):
     The cyclic garbage collector is emptied first and held off until capture_end: a dead ChunkGraphs <-> model cycle of an
     earlier signature owns CUDAGraph objects and pool memory, and torch 2.10's torch.cuda.graph no longer collects before a
     capture -- their destructors running on whichever thread trips the collector mid-capture abort the process
-    (gpurun_out r4r: "Fatal Python error: Aborted / Garbage-collecting" inside graphs.capture, 5 of 5 runs on one box)."""
+    ("Fatal Python error: Aborted / Garbage-collecting" inside graphs.capture, 5 of 5 runs on one box)."""
     _gc_was_on[0] = _gc.isenabled()
     _gc.collect()
     _gc.disable()
