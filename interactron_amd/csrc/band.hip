@@ -354,12 +354,14 @@ constexpr float kFirstF = 1099511627776.f;   // 2^40
 // tiles.  f32, 16 x 361 of 8 heads of 32, window 64: 20 us = 52 of 154 TFLOP/s, matrix pipe 40 %, vector instructions 23 %, and of the LDS cycles
 // a quarter bank conflicts: six short tiles a workgroup do not cover their waits.
 constexpr float kSlack = 8.f;
-// fp16: weights are carried 2^7 and, for dv, 2^12 times as large (the largest forward weight, 2^8 by the slack, is then 2^15; the type ends at
-// 65 504), so that its smallest step, 2^-24, is 2^-31 of the row's largest weight and 2^-36: a row whose first key takes nearly all the weight
-// keeps what the others have.
+// fp16: weights are carried 2^7 and, for dv, 2^10 times as large (the largest forward weight, 2^8 by the slack, is then 2^15; the type ends at
+// 65 504), so that its smallest step, 2^-24, is 2^-31 of the row's largest weight and 2^-34: a row whose first key takes nearly all the weight
+// keeps what the others have.  Where exponents are so large that a float32 does not hold them to less than a step (kWide), a weight can come
+// out beyond 2^15: it is cut there (a select, which a NaN passes), in a branch that other rows do not take.
 template <int DT> constexpr float kUp = DT == 2 ? 7.f : 0.f;
 template <int DT> constexpr float kUpFactor = DT == 2 ? 128.f : 1.f;
-template <int DT> constexpr float kUpDv = DT == 2 ? 4096.f : 1.f;
+template <int DT> constexpr float kUpDv = DT == 2 ? 1024.f : 1.f;
+constexpr float kWide = 1048576.f;   // 2^20: steps of 2^-3
 
 template <int DT, int D, int NB, int TB>
 __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) {
@@ -456,10 +458,19 @@ __device__ __forceinline__ void band_fwd(const BandArgs& a, unsigned char* mem) 
 #pragma unroll
                     for (int sb = 0; sb < SB; ++sb)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            s[nb][sb][r] = seq_exp2(fmaf(s[nb][sb][r], a.c2, -ref));
-                            sum[nb] += s[nb][sb][r];
+                        for (int r = 0; r < 4; ++r) s[nb][sb][r] = seq_exp2(fmaf(s[nb][sb][r], a.c2, -ref));
+                    if constexpr (DT == 2) {
+                        if (__builtin_amdgcn_ballot_w64(fabsf(ref) > kWide)) {
+#pragma unroll
+                            for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) s[nb][sb][r] = s[nb][sb][r] > 32768.f ? 32768.f : s[nb][sb][r];
                         }
+                    }
+#pragma unroll
+                    for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sum[nb] += s[nb][sb][r];
                 }
                 // 32-row steps whose columns come in one block of reads (head dim 128: four column blocks of one step; more at once was no faster)
                 constexpr int KK = SB / 2, TOGETHER = I::DB == 8 ? 1 : KK;
